@@ -133,6 +133,17 @@ HIP_SYMBOLS = {
                                          C.c_int, vp, vp, C.c_int, vp, vp, i64, vp, vp, vp]),
     "bx_qk_rope_kv_rows_f16": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_float, vp, vp,
                                          vp, C.c_int, vp, vp, vp, i64, vp, vp]),
+    "bx_kv_plan_workspace_bytes": (C.c_size_t, []),
+    "bx_kv_plan": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, C.c_int, vp,
+                             vp, C.c_size_t, vp]),
+    "bx_kv_append_q8_f16": (C.c_int, [vp, i64, vp, i64, C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp,
+                                      vp, vp]),
+    "bx_kv_read_q8_f16": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, i64, vp, i64,
+                                    vp]),
+    "bx_attention_paged_q8_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
+    "bx_attention_paged_q8_f16": (C.c_int, [vp, i64, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int,
+                                            C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64, vp,
+                                            C.c_size_t, vp]),
     "bx_linear_group_f16": (C.c_int, [C.c_int, C.c_int, C.POINTER(vp), C.POINTER(vp), C.POINTER(C.c_int), vp, C.c_int,
                                       C.c_int, vp, C.c_size_t, vp]),
     "bx_linear_residual_f16": (C.c_int, [C.c_int, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),

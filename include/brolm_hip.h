@@ -298,6 +298,90 @@ int bx_masked_mean_pool_f16(const uint16_t* x, const float* mask, int L, int col
 /* FP32 -> FP16 copy (RNE). */
 int bx_f32_to_f16(const float* x, uint16_t* y, int64_t n, void* stream);
 
+/* ------------------------------------------------------- paged 8-bit cache */
+
+/* The KV cache of several sequences in pages, in 8 bits (an extension of the
+ * one-sequence FP16 cache of dense_decoder.cpp:196-227; no counterpart in the
+ * reference).  A page holds `page` (16, 32, 64 or 128) tokens of every KV head:
+ *   Kc  int8 (n_pages, n_kv, page, hd)      k_scale  FP32 (n_pages, n_kv)
+ *   Vc  int8 (n_pages, n_kv, hd, page)      v_scale  FP32 (n_pages, n_kv)
+ * value = code * scale, codes in [-127, 127]; hd 64, 128 or 256; Kc and Vc on 16
+ * bytes.  A token's slot is its page * page + its place in the page; a request's
+ * block table (a row of `table`, int32) names the page of its tokens [b page,
+ * (b + 1) page).  Memory need not be cleared before its first use.
+ *
+ * One step of a batch: bx_kv_plan, then per layer bx_kv_append_q8_f16 and
+ * bx_attention_paged_q8_f16 with the layer's own pages (the table is shared by
+ * the layers; positions and slots also fit bx_rope_rows_f16 and
+ * bx_kv_append_rows_f16).  All arrays are device memory. */
+
+/* What bx_kv_plan's status word reports; 0: the step was laid out. */
+#define BX_KV_PLAN_NO_PAGES 1    /* fewer free pages than the step needs */
+#define BX_KV_PLAN_TABLE_FULL 2  /* a request would outgrow its table row */
+#define BX_KV_PLAN_ROWS_FULL 4   /* more than max_rows new tokens */
+#define BX_KV_PLAN_BAD_LENGTH 8  /* a negative length, or more given back than held */
+#define BX_KV_PLAN_BAD_RING 16   /* ring ends that no pool of n_pages can have */
+
+/* Lays out one step of n_req (<= 4096) requests: request r holds past[r] tokens and
+ * gets delta[r] new ones (0: none) or gives -delta[r] of its last ones back.
+ *   lens[r] = past[r] + delta[r]; starts[r] (n_req + 1): first row of request r
+ *   among the step's new tokens, starts[n_req] their number; pos[i], slots[i]: position and
+ *   slot of row i, -1 for the rows behind the last one up to max_rows (a slot is
+ *   -1 too where a table or ring entry names no page of the pool).
+ * Free pages wait in a ring of n_pages entries: entry e of ends[0] <= e < ends[1]
+ * sits at ring[e mod n_pages].  Pages taken leave its head in the order of
+ * requests, then blocks, and enter the table; pages given back (those that
+ * none of the remaining tokens is in) join its tail in the same order.  Other
+ * table entries stay as they are.  A new pool: ring[i] = i, ends = {0, n_pages}.
+ * When *status is not 0, nothing else changes: lens = past, ends_out = ends_in,
+ * every slot and position -1, every starts 0 (the step's other calls then do
+ * nothing).  lens may be past and ends_out may be ends_in (the state in place).
+ * ws: bx_kv_plan_workspace_bytes() bytes, 8-byte aligned, zeroed once before its
+ * first use; calls sharing one must not overlap. */
+size_t bx_kv_plan_workspace_bytes(void);
+int bx_kv_plan(const int32_t* past, const int32_t* delta, int n_req, int page, int n_pages, int32_t* table,
+               int max_blocks, int32_t* ring, const int64_t* ends_in, int64_t* ends_out, int32_t* lens, int32_t* starts,
+               int64_t* slots, int32_t* pos, int max_rows, int32_t* status, void* ws, size_t ws_bytes, void* stream);
+
+/* Rows of k and v (rows, n_kv*hd) FP16, k_stride / v_stride elements apart, into
+ * their slots; rows whose slot lies outside the pool are skipped.  Rows of one
+ * page stand together, in order of their slots (as bx_kv_plan lays them out):
+ * two such groups for one page in one call would race.  The tokens of the page
+ * before the group's first one are kept, what lies behind it is not.  Per page
+ * and head the scale becomes max(scale, amax / 127) (amax / 127 where the group
+ * starts the page); where it grew, the kept codes c are rounded anew, rint(c *
+ * old / new); new codes are rint(x / scale).  A NaN or an infinity makes the
+ * scale, and with it every value of that page and head, NaN or infinite. */
+int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride, int rows, int n_kv,
+                        int hd, const int64_t* slots, int page, int n_pages, int8_t* Kc, int8_t* Vc, float* k_scale,
+                        float* v_scale, void* stream);
+
+/* The rows at `slots`, as FP16: k and v (rows, n_kv*hd), k_stride / v_stride
+ * elements apart (to move a request to another pool or to the FP16 cache).  Rows
+ * whose slot lies outside the pool are left as they are. */
+int bx_kv_read_q8_f16(const int64_t* slots, int rows, int n_kv, int hd, int page, int n_pages, const int8_t* Kc,
+                      const int8_t* Vc, const float* k_scale, const float* v_scale, uint16_t* k, int64_t k_stride,
+                      uint16_t* v, int64_t v_stride, void* stream);
+
+/* Attention over the paged cache, prompt chunks and single tokens in one call: the
+ * rows starts[r] .. starts[r + 1] - 1 of q (rows, n_q*hd), q_stride elements apart,
+ * are the last positions of request r's lens[r] keys; a row at position p attends
+ * keys [max(0, p - window + 1), p] (window 0: all up to p), scores q k / sqrt(hd)
+ * -> out (rows, n_q*hd), out_stride apart.  Query head h reads KV head h / (n_q /
+ * n_kv), n_q / n_kv <= 16.  Rows from starts[n_req] on are left as they are; a row
+ * that sees no key (more rows than keys; table entries that name no page hide
+ * their keys) gives zeros.  max_new >= every request's rows (rows past max_new
+ * may be left as they are) and max_len (about the longest request) shape the launch.
+ * ws: bx_attention_paged_q8_workspace_bytes(...) bytes with the same arguments,
+ * 16-byte aligned, zeroed once before its first use; calls sharing one must not
+ * overlap. */
+size_t bx_attention_paged_q8_workspace_bytes(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len);
+int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, const int32_t* starts, const int32_t* lens,
+                              int n_req, int max_new, int max_len, const int32_t* table, int max_blocks, int page,
+                              int n_pages, const int8_t* Kc, const int8_t* Vc, const float* k_scale,
+                              const float* v_scale, int n_q, int n_kv, int hd, int window, uint16_t* out,
+                              int64_t out_stride, void* ws, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------ decode step */
 
 /* Fused single-token decode kernels (the captured step of
