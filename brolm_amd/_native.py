@@ -133,6 +133,7 @@ HIP_SYMBOLS = {
                                          C.c_int, vp, vp, C.c_int, vp, vp, i64, vp, vp, vp]),
     "bx_qk_rope_kv_rows_f16": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_float, vp, vp,
                                          vp, C.c_int, vp, vp, vp, i64, vp, vp]),
+    "bx_sample_rows_f16": (C.c_int, [vp, i64, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp]),
     "bx_kv_plan_workspace_bytes": (C.c_size_t, []),
     "bx_kv_plan": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, C.c_int, vp,
                              vp, C.c_size_t, vp]),

@@ -290,6 +290,20 @@ int bx_sample_feed_f16(const uint16_t* logits, int vocab, float temperature, int
                        void* stream);
 int bx_sample_f16(const uint16_t* logits, int vocab, float temperature, int top_k, float top_p, double u,
                   int32_t* out, void* workspace, void* stream);
+/* sample_token (generate.cpp:68-142) for every row of a batched step's logits
+ * (rows, vocab) FP16, `stride` elements apart, in one launch without a workspace; each
+ * row has its own settings and random number (device arrays of `rows`;
+ * top_k, top_p and min_p may be NULL: no such cut).  Ids stand in order of their
+ * logit, equal ones by ascending id.  Kept are the ids that are among the first
+ * top_k (<= 0: all), whose probability is at least min_p times the largest, and
+ * before which less than top_p of the whole mass stands (>= 1: no such cut); the
+ * first id stays in any case.  Drawn is the first id where the running kept mass
+ * exceeds u (in [0, 1)) times the kept mass; masses in FP64 from the exact logits /
+ * temperature.  A temperature that is not positive takes the first id.  NaN
+ * logits count as -infinity; out (rows) device int32.  vocab <= 4,194,304. */
+int bx_sample_rows_f16(const uint16_t* logits, int64_t stride, int rows, int vocab, const float* temperature,
+                       const int32_t* top_k, const float* top_p, const float* min_p, const double* u, int32_t* out,
+                       void* stream);
 /* masked_mean_pool_forward(x, mask, out) (src/llm2vec.cpp:139-153): out[c] =
  * sum_r mask[r] x[r, c] / sum_r mask[r] over the L rows of x (L, cols) FP16,
  * FP32 sums, FP16 out (cols); mask (device FP32, L) or NULL for all rows; an

@@ -82,3 +82,15 @@ def test_attention_workspace_query(native):
     assert f(0, 1, 16, 8, 128, 1, 100) == 0 and f(1, 1, 15, 8, 128, 1, 100) == 0
     assert f(1, 1, 16, 8, 128, 1, 100) > 0
     assert f(1, 1, 16, 8, 128, 1, 100000) > f(1, 1, 16, 8, 128, 1, 100)
+
+
+SAMPLE = [("logits", P), ("stride", 1000), ("rows", 4), ("vocab", 1000), ("t", P), ("k", None), ("p", None),
+          ("m", None), ("u", P), ("out", P), ("stream", None)]
+
+
+@pytest.mark.parametrize("kw,code,word", [
+    (dict(logits=None), EINVAL, "null"), (dict(t=None), EINVAL, "null"), (dict(u=None), EINVAL, "null"),
+    (dict(out=None), EINVAL, "null"), (dict(rows=0), EINVAL, "shape"), (dict(vocab=0), EINVAL, "shape"),
+    (dict(stride=999), EINVAL, "shape"), (dict(vocab=4194305, stride=1 << 23), EUNSUPPORTED, "4194304")])
+def test_sample_rows_refuses(native, kw, code, word):
+    _refused(native, "bx_sample_rows_f16", _with(SAMPLE, **kw), code, word)
