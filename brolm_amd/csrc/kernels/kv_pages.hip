@@ -7,6 +7,8 @@
 // bytes along hd for Q K^T, 16 bytes along the tokens for P V) are plain 16-byte
 // loads.  One FP32 scale per page, head and matrix: value = code * scale, codes
 // in [-127, 127].
+#include <type_traits>
+
 #include "kv_pages.h"
 
 namespace bx {
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
 //
 // A run is a row whose predecessor in the call is not the token before it in the
 // same page, with the rows after it that are: the tokens that one page receives.
-// One wavefront writes a run of one head, of K or of V:
+// Per run, head and matrix:
 //   amax over the run, s = max(s_old, amax / 127) (s_old = 0 for a page that was
 //   empty); where s grew, the page's earlier codes c become rint(c s_old / s); the
 //   new codes are rint(x / s).
@@ -185,9 +187,17 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
 // exact in FP32 (x and q s are multiples of s's last place, and the remainder is
 // below s), the earlier codes' quotient is formed in FP64, where c s_old is exact.
 // |x| is compared as the FP16 bit pattern, which orders NaN last: a page with a
-// NaN or an infinity gets such a scale, and every value of it becomes NaN.
+// NaN or an infinity gets such a scale, and every value of it becomes NaN or infinite.
+//
+// A wavefront's unit is 16 tokens of one head, in registers from the one load to
+// the store: of K a lane holds 8 head dims of hd / 32 tokens, of V 4 head dims of hd /
+// 16 consecutive tokens, which are consecutive bytes of the token-minor page.  Every
+// byte is read, requantized and written by one lane.  The four wavefronts of a
+// workgroup are the units of a page (and of 4 / (units) heads where a page has
+// fewer), which share its amax through LDS.
 
 typedef u4v __attribute__((aligned(2))) any16;
+typedef u2v __attribute__((aligned(2))) any8;
 
 struct AppendArgs {
     const uint16_t* x[2];   // K rows, V rows
@@ -201,13 +211,11 @@ struct AppendArgs {
 
 // rint(x / s), ties to even; inv is about 1 / s, s > 0 and finite.
 __device__ __forceinline__ int q8_code(float x, float s, float inv) {
-    float q = rintf(x * inv);
-    const float r = __builtin_fmaf(-q, s, x), h = 0.5f * s;
-    // one step off at most: the remainder says which way (equal: the even one)
-    const bool odd = ((int)q & 1) != 0;
-    if (r > h || (r == h && odd)) q += 1.f;
-    else if (r < -h || (r == -h && odd)) q -= 1.f;
-    return (int)q;
+    const float q = rintf(x * inv);
+    const float r = __builtin_fmaf(-q, s, x), a = fabsf(r), h = 0.5f * s;
+    // one step off at most: the remainder says whether and which way (equal: the even one)
+    const bool off = (a > h) | ((a == h) & (((int)q & 1) != 0));
+    return (int)q + (off ? (r > 0.f ? 1 : -1) : 0);
 }
 
 __device__ __forceinline__ uint32_t pk_max_abs(uint32_t m, uint32_t x) {
@@ -216,123 +224,199 @@ __device__ __forceinline__ uint32_t pk_max_abs(uint32_t m, uint32_t x) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
 }
 
-// The earlier codes of four bytes, requantized: those of tokens below `keep` (byte i
-// holds token t0 + i); others as they are.
-__device__ __forceinline__ int requant(int c, float s_old, float s_new) {
-    return (int)rint((double)c * (double)s_old / (double)s_new);
+__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int8_t)(w >> (8 * i)); }
+__device__ __forceinline__ uint32_t put_byte(uint32_t w, int i, int c) {
+    return (w & ~(0xffu << (8 * i))) | ((uint32_t)(c & 0xff) << (8 * i));
 }
 
-template <int HD>
-__device__ void append_run(const AppendArgs& a, int row, int n, int head, int which) {
-    constexpr int CH = HD / 8;        // 16-byte pieces of a row
-    constexpr int RP = 64 / CH > 0 ? 64 / CH : 1;   // rows a wavefront reads at once
-    const int lane = threadIdx.x & 63, page = 1 << a.pshift;
-    const int64_t slot = a.slots[row], pg = slot >> a.pshift;
+// WHICH 0: K, 1: V; NCH units of 16 tokens a page.
+template <int HD, int WHICH, int NCH>
+__device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, int64_t slot, uint32_t* red) {
+    constexpr int HPW = NCH < 4 ? 4 / NCH : 1;   // heads a workgroup takes
+    constexpr int U = NCH > 4 ? NCH / 4 : 1;     // units a wavefront takes
+    constexpr int page = 16 * NCH;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hs = NCH < 4 ? wave / NCH : 0;
+    const int head = (int)blockIdx.y * HPW + hs;
+    const bool there = head < a.n_kv;
     const int off = (int)(slot & (page - 1));
-    const int64_t hp = pg * a.n_kv + head;
-    const uint16_t* const x = a.x[which] + (int64_t)row * a.stride[which] + (int64_t)head * HD;
-    const int64_t st = a.stride[which];
-    float* const sp = a.scale[which] + hp;
-    int8_t* const codes = a.codes[which] + hp * page * HD;
-    const uint32_t old_bits = off > 0 ? __float_as_uint(*sp) : 0u;
+    const int64_t hp = (slot >> a.pshift) * a.n_kv + (there ? head : 0);
+    const int64_t st = a.stride[WHICH];
+    // row of token tk of the page: x + tk st
+    const uint16_t* const x = a.x[WHICH] + ((int64_t)row - off) * st + (int64_t)head * HD;
+    float* const sp = a.scale[WHICH] + hp;
+    int8_t* const codes = a.codes[WHICH] + hp * page * HD;
+    const uint32_t old_bits = off > 0 && there ? __float_as_uint(*sp) : 0u;
+    // K: piece j of a lane is token kt + j KR, head dims kd ..; V: row j of a lane is
+    // token vt + j, head dims vd .. vd + 3
+    constexpr int KL = HD / 32, KR = 512 / HD, VT = HD / 16;
+    const int kt = lane / (HD / 8), kd = 8 * (lane % (HD / 8));
+    const int vt = lane / (HD / 4) * VT, vd = 4 * (lane % (HD / 4));
+    u4v kx[U][KL];
+    u2v vx[U][VT];
+    uint32_t old[U][4][VT / 4];   // V: the lane's bytes of 4 head dims
     uint32_t m2 = 0u;
-    for (int i = lane / CH; i < n; i += RP) {
-        const u4v w = *reinterpret_cast<const any16*>(x + (int64_t)i * st + 8 * (lane % CH));
-        m2 = pk_max_abs(pk_max_abs(pk_max_abs(pk_max_abs(m2, w.x), w.y), w.z), w.w);
+    auto fresh = [&](int tk) { return tk >= off && tk < off + n; };
+    auto v_piece = [&](int c, int d) { return codes + (int64_t)(vd + d) * page + 16 * c + vt; };
+    auto load_old = [&](int u, int c) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const uint32_t* const p = reinterpret_cast<const uint32_t*>(v_piece(c, d));
+#pragma unroll
+            for (int i = 0; i < VT / 4; ++i) old[u][d][i] = p[i];
+        }
+    };
+    bool has_new[U], part[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = (NCH < 4 ? wave % NCH : wave) + 4 * u, t0 = 16 * c;
+        has_new[u] = there && t0 < off + n && t0 + 16 > off;
+        part[u] = has_new[u] && WHICH == 1 && !(t0 + vt >= off && t0 + vt + VT <= off + n);
+        // tokens outside the run read its nearest row and count as zero: loads without
+        // branches between them
+        auto near = [&](int tk) { return x + (int64_t)min(max(tk, off), off + n - 1) * st; };
+        if constexpr (WHICH == 0) {
+            if (has_new[u]) {
+#pragma unroll
+                for (int j = 0; j < KL; ++j) kx[u][j] = *reinterpret_cast<const any16*>(near(t0 + kt + j * KR) + kd);
+#pragma unroll
+                for (int j = 0; j < KL; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        m2 = pk_max_abs(m2, kx[u][j][i] & (fresh(t0 + kt + j * KR) ? 0xffffffffu : 0u));
+            }
+        } else if (has_new[u]) {
+            if (part[u]) load_old(u, c);
+#pragma unroll
+            for (int j = 0; j < VT; ++j) vx[u][j] = *reinterpret_cast<const any8*>(near(t0 + vt + j) + vd);
+#pragma unroll
+            for (int j = 0; j < VT; ++j) {
+                const uint32_t in = fresh(t0 + vt + j) ? 0xffffffffu : 0u;
+                m2 = pk_max_abs(pk_max_abs(m2, vx[u][j].x & in), vx[u][j].y & in);
+            }
+        }
     }
     uint32_t m = max(m2 & 0xffffu, m2 >> 16);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    if constexpr (NCH > 1) {
+        if (lane == 0) red[wave] = m;
+        __syncthreads();
+        m = 0u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            if (NCH >= 4 || w / NCH == hs) m = max(m, red[w]);
+    }
+    if (!there) return;
     const uint32_t new_bits = max(old_bits, __float_as_uint(h2f((uint16_t)m) / 127.0f));
     const float s_old = __uint_as_float(old_bits), s = __uint_as_float(new_bits);
     const bool live = s > 0.f && s < INFINITY;   // else every code is 0
-    const float inv = live ? 1.0f / s : 0.f;
-    if (lane == 0) *sp = s;
-    auto code = [&](uint16_t h) { return live ? q8_code(h2f(h), s, inv) : 0; };
+    const float div = live ? s : INFINITY, inv = live ? 1.0f / s : 0.f;
     const bool grew = off > 0 && new_bits != old_bits;
-    auto moved = [&](int c) { return live ? requant(c, s_old, s) : 0; };
-    if (which == 0) {
-        if (grew) {
-            u4v* const p = reinterpret_cast<u4v*>(codes);
-            for (int i = lane; i < off * HD / 16; i += 64) {
-                u4v w = p[i];
+    if ((NCH < 4 ? wave % NCH : wave) == 0 && lane == 0) *sp = s;
+    // the codes of four values, half h of each of four dwords
+    auto code4 = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int h0, int h1, int h2, int h3) {
+        auto one = [&](uint32_t w, int h) { return (uint32_t)q8_code(h2f((uint16_t)(w >> (16 * h))), div, inv) & 0xffu; };
+        return one(w0, h0) | (one(w1, h1) << 8) | (one(w2, h2) << 16) | (one(w3, h3) << 24);
+    };
+    // the earlier codes of one dword, the first of them token tk's and the others
+    // `step` tokens apart, requantized in place
+    auto move4 = [&](uint32_t* p, int tk, int step) {
+        uint32_t y = *p;
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b)
+            if (tk + b * step < off)
+                y = put_byte(y, b, live ? (int)rint((double)byte_of(y, b) * (double)s_old / (double)s) : 0);
+        *p = y;
+    };
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t y = 0u;
-#pragma unroll
-                    for (int b = 0; b < 4; ++b)
-                        y |= (uint32_t)(moved((int8_t)(w[j] >> (8 * b))) & 0xff) << (8 * b);
-                    w[j] = y;
+    for (int u = 0; u < U; ++u) {
+        const int c = (NCH < 4 ? wave % NCH : wave) + 4 * u, t0 = 16 * c;
+        if (grew && t0 < off) {
+            if constexpr (WHICH == 0) {
+#pragma unroll 1
+                for (int j = 0; j < 2 * KL; ++j) {
+                    const int tk = t0 + kt + j / 2 * KR;
+                    if (tk < off) move4(reinterpret_cast<uint32_t*>(codes + tk * HD + kd) + (j & 1), tk, 0);
                 }
-                p[i] = w;
+            } else {
+#pragma unroll 1
+                for (int d = 0; d < 4; ++d)
+#pragma unroll 1
+                    for (int i = 0; i < VT / 4; ++i)
+                        if (t0 + vt + 4 * i < off) move4(reinterpret_cast<uint32_t*>(v_piece(c, d)) + i, t0 + vt + 4 * i, 1);
+                if (part[u]) load_old(u, c);
             }
         }
-        for (int i = lane / CH; i < n; i += RP) {
-            const u4v w = *reinterpret_cast<const any16*>(x + (int64_t)i * st + 8 * (lane % CH));
-            u2v y{0u, 0u};
+        if (!has_new[u]) continue;
+        if constexpr (WHICH == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                y[j / 4] |= (uint32_t)(code((uint16_t)(w[j / 2] >> (16 * (j & 1)))) & 0xff) << (8 * (j & 3));
-            *reinterpret_cast<u2v*>(codes + (int64_t)(off + i) * HD + 8 * (lane % CH)) = y;
-        }
-        return;
-    }
-    // V: pieces of 16 tokens of one head dim; a piece that also holds earlier tokens
-    // (or ones behind the run) keeps their bytes
-    for (int c0 = grew ? 0 : off & ~15; c0 < off + n; c0 += 16) {
-        const bool whole = c0 >= off && c0 + 16 <= off + n;
-        for (int d = lane; d < HD; d += 64) {
-            u4v* const p = reinterpret_cast<u4v*>(codes + (int64_t)d * page + c0);
-            u4v w{0u, 0u, 0u, 0u};
-            if (!whole) w = *p;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int tk = c0 + j, sh = 8 * (j & 3);
-                int y = (int8_t)(w[j / 4] >> sh);
-                if (tk >= off && tk < off + n) y = code(x[(int64_t)(tk - off) * st + d]);
-                else if (grew && tk < off) y = moved(y);
-                w[j / 4] = (w[j / 4] & ~(0xffu << sh)) | ((uint32_t)(y & 0xff) << sh);
+            for (int j = 0; j < KL; ++j) {
+                const int tk = t0 + kt + j * KR;
+                if (fresh(tk)) {
+                    const u4v w = kx[u][j];
+                    *reinterpret_cast<u2v*>(codes + tk * HD + kd) =
+                        u2v{code4(w.x, w.x, w.y, w.y, 0, 1, 0, 1), code4(w.z, w.z, w.w, w.w, 0, 1, 0, 1)};
+                }
             }
-            *p = w;
+        } else if (t0 + vt < off + n && t0 + vt + VT > off) {   // new tokens among the lane's
+#pragma unroll
+            for (int i = 0; i < VT / 4; ++i) {
+                // bytes of the run's tokens
+                const int tk = t0 + vt + 4 * i, lo = min(4, max(0, off - tk)), hi = min(4, max(0, off + n - tk));
+                const uint32_t keep = ~(hi > lo ? (0xffffffffu >> (8 * (4 - hi + lo))) << (8 * lo) : 0u);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t y = code4(vx[u][4 * i][d / 2], vx[u][4 * i + 1][d / 2], vx[u][4 * i + 2][d / 2],
+                                             vx[u][4 * i + 3][d / 2], d & 1, d & 1, d & 1, d & 1);
+                    old[u][d][i] = part[u] ? (old[u][d][i] & keep) | (y & ~keep) : y;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < VT / 4; ++i) reinterpret_cast<uint32_t*>(v_piece(c, d))[i] = old[u][d][i];
         }
     }
 }
 
-template <int HD>
-__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
-    // wavefront -> (window of rows, head, K or V); the runs that start in its window
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int which = (int)(item & 1), head = (int)((item >> 1) % a.n_kv);
-    const int64_t row0 = (item >> 1) / a.n_kv * a.window;
-    const int lane = threadIdx.x & 63, page = 1 << a.pshift;
-    if (row0 >= a.rows) return;
+// Workgroup (window of rows, heads, K or V): the runs that start in its window, one
+// after the other.
+template <int HD, int NCH>
+__global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(AppendArgs a) {
+    __shared__ uint32_t red[2][4];
+    const int64_t row0 = (int64_t)blockIdx.x * a.window;
+    const int lane = threadIdx.x & 63;
+    constexpr int page = 16 * NCH;
     auto slot_at = [&](int64_t r) { return r >= 0 && r < a.rows ? a.slots[r] : -1; };
-    const int64_t r = row0 + lane;
-    const int64_t own = slot_at(r), prev = slot_at(r - 1);
+    const int64_t r = row0 + lane, own = slot_at(r), prev = slot_at(r - 1);
     const bool first = lane < a.window && own >= 0 && own < a.n_slots && ((own & (page - 1)) == 0 || own != prev + 1);
     uint64_t todo = __ballot(first);
-    while (todo) {
+    for (int k = 0; todo; k ^= 1) {   // red alternates: one barrier a run
         const int i = __builtin_ctzll(todo);
         todo &= todo - 1;
         const int row = (int)(row0 + i);
         const int64_t slot = a.slots[row];
         const int left = page - (int)(slot & (page - 1));   // tokens to the page's end
         int n = 0;
-        for (int k = 0; k < left; k += 64) {
-            const uint64_t same = __ballot(k + lane < left && slot_at((int64_t)row + k + lane) == slot + k + lane);
+        for (int q = 0; q < left; q += 64) {
+            const uint64_t same = __ballot(q + lane < left && slot_at((int64_t)row + q + lane) == slot + q + lane);
             const int c = ~same ? __builtin_ctzll(~same) : 64;
             n += c;
             if (c < 64) break;
         }
-        append_run<HD>(a, row, n, head, which);
+        if (blockIdx.z == 0) append_run<HD, 0, NCH>(a, row, n, slot, red[k]);
+        else append_run<HD, 1, NCH>(a, row, n, slot, red[k]);
     }
 }
 
 // ------------------------------------------------------------------ the read
 //
-// A wavefront takes 16 rows of one head, of K or of V.  K rows are 16-byte loads;
-// V, token-minor, is read in 16-byte pieces of 16 tokens of a head dim where the
-// rows are consecutive tokens of one page, else byte by byte.
+// A wavefront takes 16 rows of one head.  Of K a lane reads 16 codes of a row.  Of V
+// it takes the pieces of 16 tokens of a page that begin among its rows (a row that
+// is not the next token of the row before it, or the first of a piece): a lane holds
+// 4 head dims of hd / 16 tokens.
 struct ReadArgs {
     const int64_t* slots;
     int rows, n_kv, pshift;
@@ -343,7 +427,9 @@ struct ReadArgs {
     int64_t stride[2];
 };
 
-__device__ __forceinline__ uint16_t q8_value(int c, float s) { return f2h(f32_fence((float)c * s)); }
+__device__ __forceinline__ uint32_t q8_pair(int c0, int c1, float s) {
+    return (uint32_t)f2h(f32_fence((float)c0 * s)) | ((uint32_t)f2h(f32_fence((float)c1 * s)) << 16);
+}
 
 template <int HD>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
@@ -352,16 +438,70 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
     const int64_t row0 = (item >> 1) / a.n_kv * 16;
     const int lane = threadIdx.x & 63, page = 1 << a.pshift;
     if (row0 >= a.rows) return;
-    const int n = (int)min((int64_t)16, a.rows - row0);
-    for (int i = 0; i < n; ++i) {
-        const int64_t slot = a.slots[row0 + i];
-        if (slot < 0 || slot >= a.n_slots) continue;
+    auto slot_at = [&](int64_t r) { return r >= 0 && r < a.rows ? a.slots[r] : -1; };
+    if (which == 0) {
+        constexpr int LR = HD / 16, RP = 64 / LR;   // lanes a row, rows at once
+        int64_t slot[16 / RP];
+        u4v w[16 / RP];
+        float s[16 / RP];
+#pragma unroll
+        for (int j = 0; j < 16 / RP; ++j) {
+            slot[j] = slot_at(row0 + j * RP + lane / LR);
+            if (slot[j] >= a.n_slots) slot[j] = -1;
+        }
+#pragma unroll
+        for (int j = 0; j < 16 / RP; ++j) {
+            const int64_t at = slot[j] < 0 ? 0 : slot[j], hp = (at >> a.pshift) * a.n_kv + head;
+            w[j] = *gptr<u4v>(a.codes[0] + (hp * page + (at & (page - 1))) * HD + 16 * (lane % LR));
+            s[j] = a.scale[0][hp];
+        }
+#pragma unroll
+        for (int j = 0; j < 16 / RP; ++j) {
+            if (slot[j] < 0) continue;
+            any16* const y = reinterpret_cast<any16*>(a.y[0] + (row0 + j * RP + lane / LR) * a.stride[0] +
+                                                      (int64_t)head * HD + 16 * (lane % LR));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u4v z;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t b = w[j][2 * h + i / 2];
+                    z[i] = q8_pair(byte_of(b, 2 * (i & 1)), byte_of(b, 2 * (i & 1) + 1), s[j]);
+                }
+                y[h] = z;
+            }
+        }
+        return;
+    }
+    const int64_t own = slot_at(row0 + lane), prev = slot_at(row0 + lane - 1);
+    const bool first = lane < 16 && own >= 0 && own < a.n_slots && ((own & 15) == 0 || own != prev + 1);
+    uint64_t todo = __ballot(first);
+    constexpr int VT = HD / 16;
+    const int vt = lane / (HD / 4) * VT, vd = 4 * (lane % (HD / 4));
+    while (todo) {
+        const int i = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int64_t slot = __shfl(own, i);
+        const int o = (int)(slot & 15);   // its place in the piece
+        const uint64_t same = __ballot(lane < 16 - o && slot_at(row0 + i + lane) == slot + lane);
+        const int n = __builtin_ctzll(~same);
         const int64_t hp = (slot >> a.pshift) * a.n_kv + head;
-        const int off = (int)(slot & (page - 1));
-        const float s = a.scale[which][hp];
-        const int8_t* const c = a.codes[which] + hp * page * HD;
-        uint16_t* const y = a.y[which] + (row0 + i) * a.stride[which] + (int64_t)head * HD;
-        for (int d = lane; d < HD; d += 64) y[d] = q8_value(which ? c[(int64_t)d * page + off] : c[off * HD + d], s);
+        const int8_t* const p = a.codes[1] + (hp * HD + vd) * page + ((slot & (page - 1)) - o) + vt;
+        const float s = a.scale[1][hp];
+        uint32_t w[4][VT / 4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int q = 0; q < VT / 4; ++q) w[d][q] = reinterpret_cast<const uint32_t*>(p + d * page)[q];
+#pragma unroll
+        for (int j = 0; j < VT; ++j) {
+            const int tk = vt + j;
+            if (tk < o || tk >= o + n) continue;
+            u2v z;
+            z.x = q8_pair(byte_of(w[0][j / 4], j % 4), byte_of(w[1][j / 4], j % 4), s);
+            z.y = q8_pair(byte_of(w[2][j / 4], j % 4), byte_of(w[3][j / 4], j % 4), s);
+            *reinterpret_cast<any8*>(a.y[1] + (row0 + i + tk - o) * a.stride[1] + (int64_t)head * HD + vd) = z;
+        }
     }
 }
 
@@ -423,14 +563,22 @@ int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, 
     a.rows = rows; a.n_kv = n_kv; a.pshift = __builtin_ctz((unsigned)page);
     a.n_slots = (int64_t)n_pages * page;
     a.slots = slots; a.codes[0] = Kc; a.codes[1] = Vc; a.scale[0] = k_scale; a.scale[1] = v_scale;
-    a.window = rows <= 512 ? 1 : 16;
-    const int64_t items = ((int64_t)rows + a.window - 1) / a.window * n_kv * 2, blocks = (items + 3) / 4;
-    if (blocks > 0x7fffffff) return fail(BX_EUNSUPPORTED, "kv_append_q8: too many rows and heads");
-    const dim3 grid((unsigned)blocks);
+    a.window = rows <= 1024 ? 1 : 16;
+    const unsigned windows = (unsigned)((rows + a.window - 1) / a.window);
+    const int per = page < 64 ? 64 / page : 1;   // heads a workgroup takes
+    if ((n_kv + per - 1) / per > 65535) return fail(BX_EUNSUPPORTED, "kv_append_q8: too many heads");
+    const dim3 grid(windows, (unsigned)((n_kv + per - 1) / per), 2);
     hipStream_t st = as_stream(stream);
-    if (hd == 64) kv_append_kernel<64><<<grid, 256, 0, st>>>(a);
-    else if (hd == 128) kv_append_kernel<128><<<grid, 256, 0, st>>>(a);
-    else kv_append_kernel<256><<<grid, 256, 0, st>>>(a);
+    auto run = [&](auto hdc) {
+        constexpr int HD = decltype(hdc)::value;
+        if (page == 16) kv_append_kernel<HD, 1><<<grid, 256, 0, st>>>(a);
+        else if (page == 32) kv_append_kernel<HD, 2><<<grid, 256, 0, st>>>(a);
+        else if (page == 64) kv_append_kernel<HD, 4><<<grid, 256, 0, st>>>(a);
+        else kv_append_kernel<HD, 8><<<grid, 256, 0, st>>>(a);
+    };
+    if (hd == 64) run(std::integral_constant<int, 64>{});
+    else if (hd == 128) run(std::integral_constant<int, 128>{});
+    else run(std::integral_constant<int, 256>{});
     return launch_check("kv_append_q8");
 }
 
