@@ -42,6 +42,7 @@ constexpr int kQaThreads = 256;
 constexpr int kQaMaxGroup = 16;
 constexpr int kQaLazy = 8;      // the running maximum moves when exceeded by 2^8
 constexpr int kQaReserve = 7;   // 2^(8 + 7) < 65504
+constexpr int kQaMaxSplits = 256;   // their weights (16 columns) fit the LDS of the wavefronts' shares
 constexpr int kQaMinExp = 6;    // least exponent field of the reference scale
 
 struct QaArgs {
@@ -57,7 +58,7 @@ struct QaArgs {
     int n_kv, G, window;
     uint16_t* out;
     int64_t out_stride;
-    int direct, S;
+    int S;
     uint64_t* cnt;
     unsigned char* recs;
     uint32_t tag;
@@ -86,22 +87,108 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// The V scale of a lane's 16 keys relative to the reference, times 2^kQaReserve: the factor
+// that P carries into the FP16 operand.  The reference is a power of two at or above the
+// largest finite scale so far; where it moves, `rescale` gets the factor of the sums
+// made so far.  A NaN or an infinity takes no part in it (weird: some lane has one).
+struct QaScale {
+    int eref = kQaMinExp;
+    float rv;
+    bool weird;
+
+    template <class F>
+    __device__ __forceinline__ void next(float sv, F&& rescale) {
+        const bool fin = sv < INFINITY;
+        weird = __any(!fin);
+        int ev = fin ? (int)(__float_as_uint(sv) >> 23) : 0;
+        ev = max(ev, __shfl_xor(ev, 16));
+        ev = __builtin_amdgcn_readfirstlane(max(ev, __shfl_xor(ev, 32)));
+        if (ev > eref) {
+            rescale(exp2_int(eref - ev));
+            eref = ev;
+        }
+        rv = sv * exp2_int(126 + kQaReserve - eref);
+    }
+    __device__ __forceinline__ float unit() const { return exp2_int(eref - 126 - kQaReserve); }
+};
+
+// One step of the softmax for 64 keys of a column: s[t][e] are the products of q and the
+// codes of key 4 t + e of the lane's 16, f their factor in base-2 units; hide(t, e) is
+// asked where `masked`.  The running maximum moves only when exceeded by 2^kQaLazy (rescale
+// then gets the factor of O).  The weights times the V scale come out as FP16 operands;
+// the scale enters in the exponent and leaves the sum as one factor (2^-60 in the place
+// of a zero, far below FP16).
+template <class H, class F>
+__device__ __forceinline__ void qa_softmax(float (&s)[4][4], float f, bool masked, H&& hide, const QaScale& sc, float& m,
+                                           float& l, qa_h8 (&pb)[2], F&& rescale) {
+    if (masked) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = hide(t, e) ? -INFINITY : s[t][e] * f;
+        f = 1.f;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[t][e]);
+    mx = quad_max(mx * f);
+    if (__any(mx > m + (float)kQaLazy)) {
+        const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
+        rescale(al);
+        m = mn;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!sc.weird) {
+        const float r = fmaxf(sc.rv, 8.67361738e-19f), nr = nm + __builtin_amdgcn_logf(r);   // base-2 logarithm
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], f, nr));
+                ls[e] += p;
+                pb[t / 2][4 * (t % 2) + e] = (_Float16)p;
+            }
+        l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), __builtin_amdgcn_rcpf(r), l);
+    } else {   // a hidden key weighs nothing whatever its page's scale
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], f, nm));
+                ls[e] += p;
+                pb[t / 2][4 * (t % 2) + e] = s[t][e] == -INFINITY ? (_Float16)0.f : (_Float16)(p * sc.rv);
+            }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    }
+}
+
 // The query columns of a wavefront as B operands of the integer products: lane l
 // holds column l % 16, head dims 64 c + 16 (l / 16) .. of part c.
 template <int HD>
 struct QaQuery {
     qa_i4 hi[HD / 64], lo[HD / 64];
     float scale;   // q = (256 hi + lo) scale; NaN where q holds one or an infinity
+    u4v w[HD / 64][2];
 
-    __device__ __forceinline__ void load(const uint16_t* col, bool real) {
+    // the loads apart from the arithmetic: the first tile is requested between them
+    __device__ __forceinline__ void load(const uint16_t* col) {
         const int lane = threadIdx.x & 63;
-        u4v w[HD / 64][2];
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[c][i] = *reinterpret_cast<const qa_any16*>(col + 64 * c + 16 * (lane >> 4) + 8 * i);
+    }
+    __device__ __forceinline__ void split(bool real) {
         uint32_t m = 0u;
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                w[c][i] = *reinterpret_cast<const qa_any16*>(col + 64 * c + 16 * (lane >> 4) + 8 * i);
                 if (!real) w[c][i] = u4v{0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -157,37 +244,21 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
-    // ---- block -> (column tile, split, KV head), the KV head fastest: with 8 of
-    // them an XCD keeps to one, and the tiles of a request share its L2
+    // ---- block -> (request, split, KV head)
     const int g = (int)(blockIdx.x % (unsigned)a.n_kv);
     const int64_t rest = blockIdx.x / (unsigned)a.n_kv;
     const int s = (int)(rest % a.S);
     const int64_t tile = rest / a.S;
-    int r = (int)tile, ti = 0;
-    if (!a.direct) {
-        // request r owns the tiles from starts[r] G / 16 + r on (at least as many as
-        // its columns fill)
-        int lo = 0, hi = a.n_req;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((int64_t)a.starts[mid] * G / 16 + mid <= tile) lo = mid;
-            else hi = mid;
-        }
-        r = lo;
-        ti = (int)(tile - ((int64_t)a.starts[r] * G / 16 + r));
-    }
+    const int r = (int)tile;
     const int row0 = a.starts[r], n_new = a.starts[r + 1] - row0;
-    if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || ti < 0) return;
-    const int64_t ncol = (int64_t)n_new * G, c0 = 16 * (int64_t)ti;
-    if (c0 >= ncol) return;
-    const int cols = (int)min((int64_t)16, ncol - c0);
+    if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || (int64_t)n_new * G > 16) return;
+    const int cols = n_new * G;
     const int len = (int)min((int64_t)a.lens[r], (int64_t)a.max_blocks << a.pshift);
     // positions of the tile's first and last row, and of this lane's column
     const int p0 = len - n_new;
-    const int t_first = (int)(c0 / G), t_last = (int)((c0 + cols - 1) / G);
+    const int t_first = 0, t_last = n_new - 1;
     const bool real = lc < cols;
-    const int64_t col = c0 + (real ? lc : 0);
-    const int tok = (int)(col / G), head = g * G + (int)(col % G);
+    const int col = real ? lc : 0, tok = col / G, head = g * G + col % G;
     auto low = [&](int p) { return a.window > 0 ? max(0, p - a.window + 1) : 0; };
     const int plast = real ? p0 + tok : -1, plow = low(p0 + tok);
     const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
@@ -200,52 +271,57 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
     const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
     const int last_block = max(0, (kend - 1) >> a.pshift);
     auto entry = [&](int i, int grp) {   // page of 16 keys of tile i
-        return trow[min(((k64 + i) * 64 + 16 * grp) >> a.pshift, last_block)];
+        return *gptr<int32_t>(trow + min(((k64 + i) * 64 + 16 * grp) >> a.pshift, last_block));
     };
+    // Rows of tile i, whose pages are pk (K lanes) and pv (V lanes).  Behind the last tile
+    // every lane reads the pool's first bytes instead: the same loads in every turn of the
+    // loop, so that a wait counts exactly those of its own tile, and no traffic.
     auto fetch = [&](QaTile<HD>& x, int i, int pk, int pv) {
         const int key = (k64 + i) * 64;
+        const bool live = i < te;
         x.ok = pv >= 0 && pv < a.n_pages;
         const int64_t hk = (int64_t)(pk >= 0 && pk < a.n_pages ? pk : 0) * a.n_kv + g;
         const int64_t hv = (int64_t)(x.ok ? pv : 0) * a.n_kv + g;
-        const int8_t* const kp =
-            a.Kc + (hk * page + ((key + 16 * (lc >> 2) + (lc & 3)) & (page - 1))) * HD + 16 * lg;
+        const int64_t ko = (hk * page + ((key + 16 * (lc >> 2) + (lc & 3)) & (page - 1))) * HD + 16 * lg;
+        const int64_t vo = (hv * HD + lc) * page + ((key + 16 * lg) & (page - 1));
+        const int8_t* const kp = a.Kc + (live ? ko : 0);
+        const int8_t* const vp = a.Vc + (live ? vo : 0);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < NC; ++c) x.k[t][c] = *gptr<qa_i4>(kp + 4 * t * HD + 64 * c);
-        const int8_t* const vp = a.Vc + (hv * HD + lc) * page + ((key + 16 * lg) & (page - 1));
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) x.v[j] = *gptr<u4v>(vp + (int64_t)16 * j * page);
-        x.sk = a.ks[hv];
-        x.sv = a.vs[hv];
+        for (int j = 0; j < NJ; ++j) x.v[j] = *gptr<u4v>(vp + 16 * j * page);
+        x.sk = *gptr<float>(a.ks + (live ? hv : 0));
+        x.sv = *gptr<float>(a.vs + (live ? hv : 0));
     };
 
     QaQuery<HD> qy;
     QaTile<HD> x0, x1;
-    int i0 = tb + wave;
-    int pk = 0, pv = 0;
-    if (i0 < te) {
-        pk = entry(i0, lc >> 2);
-        pv = entry(i0, lg);
-    }
-    qy.load(a.q + (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD, real);
-    if (i0 < te) fetch(x0, i0, pk, pv);
-    if (i0 + 4 < te) {
-        pk = entry(i0 + 4, lc >> 2);
-        pv = entry(i0 + 4, lg);
-    }
+    const int i0 = tb + wave;
+    int pk = entry(i0, lc >> 2), pv = entry(i0, lg);
+    qy.load(a.q + (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD);
+    const int k2 = pk, v2 = pv;
+    pk = entry(i0 + 4, lc >> 2);
+    pv = entry(i0 + 4, lg);
+    fetch(x0, i0, k2, v2);
+    __builtin_amdgcn_sched_barrier(0);
+    qy.split(real);
     const float cf = qy.scale * (1.4426950408889634f / sqrtf((float)HD));
     qa_f4 o[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) o[j] = qa_f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    int eref = kQaMinExp;
+    QaScale sc;
+    auto rescale = [&](float al) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] *= al;
+    };
 
     auto compute = [&](const QaTile<HD>& x, int i) {
-        const int key = (k64 + i) * 64;
-        // S: lane l, element r of y[t] holds key 16 (l / 16) + 4 t + r of column l % 16
+        const int key = (k64 + i) * 64, kk = key + 16 * lg;
+        // S: lane l, element e of y[t] holds key 16 (l / 16) + 4 t + e of column l % 16
         float y[4][4];
-        const float f = cf * x.sk;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             qa_i4 h{0, 0, 0, 0}, w{0, 0, 0, 0};
@@ -255,100 +331,51 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
                 w = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qy.lo[c], w, 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[t][e] = (float)(h[e] * 256 + w[e]) * f;
+            for (int e = 0; e < 4; ++e) y[t][e] = (float)(h[e] * 256 + w[e]);
+            if (t == 1) __builtin_amdgcn_sched_barrier(0);   // two fragments' integer sums at a time
         }
         const bool whole = key + 63 <= p0 + t_first && key >= low(p0 + t_last) && __all(x.ok);
-        const int kk = key + 16 * lg;
-        if (!whole) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!x.ok || kk + 4 * t + e > plast || kk + 4 * t + e < plow) y[t][e] = -INFINITY;
-        }
-        float mx = y[0][0];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, y[t][e]);
-        mx = quad_max(mx);
-        if (__any(mx > m + (float)kQaLazy)) {
-            const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            l *= al;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) o[j] *= al;
-            m = mn;
-        }
-        // the scale of V: a NaN or an infinity takes no part in the reference
-        const bool fin = x.sv < INFINITY;
-        int ev = fin ? (int)(__float_as_uint(x.sv) >> 23) : 0;
-        ev = max(ev, __shfl_xor(ev, 16));
-        ev = __builtin_amdgcn_readfirstlane(max(ev, __shfl_xor(ev, 32)));
-        if (ev > eref) {
-            const float al = exp2_int(eref - ev);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) o[j] *= al;
-            eref = ev;
-        }
-        const float rv = x.sv * exp2_int(126 + kQaReserve - eref);
-        const float nm = m == -INFINITY ? 0.f : -m;
+        sc.next(x.sv, rescale);
         qa_h8 pb[2];
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f(y[t][e] + nm);
-                ls[e] += p;
-                pb[t / 2][4 * (t % 2) + e] = (_Float16)(p * rv);
-            }
-        if (__any(!fin)) {   // a hidden key weighs nothing whatever its page's scale
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (y[t][e] == -INFINITY) pb[t / 2][4 * (t % 2) + e] = (_Float16)0.f;
-        }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        qa_softmax(
+            y, cf * x.sk, !whole,
+            [&](int t, int e) { return !x.ok || kk + 4 * t + e > plast || kk + 4 * t + e < plow; }, sc, m, l, pb, rescale);
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                u4v w;
                 uint32_t e0, e1, e2, e3;
                 codes_f16(x.v[j][2 * u], e0, e1);
                 codes_f16(x.v[j][2 * u + 1], e2, e3);
-                w = u4v{e0, e1, e2, e3};
+                const u4v w{e0, e1, e2, e3};
                 o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qa_h8, w), pb[u], o[j], 0, 0, 0);
             }
     };
-    auto next_ids = [&](int i) {
-        if (i < te) {
-            pk = entry(i, lc >> 2);
-            pv = entry(i, lg);
-        }
+    // the page ids of the tile after next are requested before the next tile's rows: loads
+    // complete in order, so ids behind the rows would hold up the fetch that needs them
+    // until the rows have come
+    auto ahead = [&](QaTile<HD>& x, int i) {
+        const int k1 = pk, v1 = pv;
+        pk = entry(i + 4, lc >> 2);
+        pv = entry(i + 4, lg);
+        fetch(x, i, k1, v1);
     };
     if constexpr (HD <= 128) {
-        for (int i = i0; i < te;) {
-            if (i + 4 < te) fetch(x1, i + 4, pk, pv);
-            next_ids(i + 8);
+        for (int i = i0; i < te; i += 8) {
+            ahead(x1, i + 4);
             compute(x0, i);
-            i += 4;
-            if (i >= te) break;
-            if (i + 4 < te) fetch(x0, i + 4, pk, pv);
-            next_ids(i + 8);
-            compute(x1, i);
-            i += 4;
+            if (i + 4 >= te) break;
+            ahead(x0, i + 8);
+            compute(x1, i + 4);
         }
     } else {   // one tile's registers
         for (int i = i0; i < te; i += 4) {
             compute(x0, i);
-            if (i + 4 < te) fetch(x0, i + 4, pk, pv);
-            next_ids(i + 8);
+            ahead(x0, i + 4);
         }
     }
     l = quad_sum(l);
-    const float unit = exp2_int(eref - 126 - kQaReserve);
+    const float unit = sc.unit();
 
     // ---- the four wavefronts' shares -> head dims j = wave, wave + 4, .. of each
     qa_f4* const so = reinterpret_cast<qa_f4*>(smem);            // [wave][j][lane]
@@ -417,58 +444,383 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
     }
     __syncthreads();
     if (!*last) return;
+    // every record's weight exp2(m - M) into LDS: lanes of group lg take the records lg, lg +
+    // 4, .. of their column; then O, sixteen records on their way at a time
+    float* const sw = reinterpret_cast<float*>(smem) + 16;   // [record][column]
+    const int mine = 8 * (real ? lc : 0);
     M = -INFINITY;
-    for (int t = 0; t < T; ++t)
-        M = fmaxf(M, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, t * kRec + NJ * 1024 + 8 * (real ? lc : 0), 0, kSc1)));
+    for (int t = lg; t < T; t += 4)
+        M = fmaxf(M, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, t * kRec + NJ * 1024 + mine, 0, kSc1)));
+    M = quad_max(M);
     L = 0.f;
+    for (int t = lg; t < T; t += 4) {
+        const u2v ml = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rs, t * kRec + NJ * 1024 + mine, 0, kSc1));
+        const float mt = __uint_as_float(ml.x), w = mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mt - M);
+        L += w * __uint_as_float(ml.y);
+        if (wave == 0) sw[t * 16 + lc] = w;
+    }
+    L = quad_sum(L);
+    __syncthreads();
 #pragma unroll
     for (int jj = 0; jj < NJ / 4; ++jj) acc[jj] = qa_f4{0.f, 0.f, 0.f, 0.f};
-    for (int t0 = 0; t0 < T; t0 += 4) {
-        u2v ml[4];
-        u4v ov[4][NJ / 4];
+    constexpr int B = 32 / (NJ / 4) > 16 ? 16 : 32 / (NJ / 4);   // records at a time
+    for (int t0 = 0; t0 < T; t0 += B) {
+        u4v ov[B][NJ / 4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int t = min(t0 + u, T - 1);
-            ml[u] = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rs, t * kRec + NJ * 1024 + 8 * (real ? lc : 0), 0, kSc1));
+        for (int u = 0; u < B; ++u)
 #pragma unroll
             for (int jj = 0; jj < NJ / 4; ++jj)
                 ov[u][jj] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(
-                                                        rs, t * kRec + (wave + 4 * jj) * 1024 + (16 * lg + (real ? lc : 0)) * 16, 0, kSc1));
-        }
+                                                        rs, min(t0 + u, T - 1) * kRec + (wave + 4 * jj) * 1024 + 256 * lg + 2 * mine,
+                                                        0, kSc1));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (t0 + u >= T) break;
-            const float mt = __uint_as_float(ml[u].x), w = mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mt - M);
-            L += w * __uint_as_float(ml[u].y);
+        for (int u = 0; u < B; ++u) {
+            const float w = t0 + u < T ? sw[(t0 + u) * 16 + lc] : 0.f;
+            if (t0 + u < T) {
 #pragma unroll
-            for (int jj = 0; jj < NJ / 4; ++jj) acc[jj] += __builtin_bit_cast(qa_f4, ov[u][jj]) * w;
+                for (int jj = 0; jj < NJ / 4; ++jj) acc[jj] += __builtin_bit_cast(qa_f4, ov[u][jj]) * w;
+            }
         }
     }
     store(L);
 }
 
-// How a call is laid out: 16 columns at most per request (direct: a tile is a
-// request) or tiles over all columns; splits of a tile's keys.
+// Prompt chunks: requests with more than 16 columns.  A workgroup takes 128 columns of
+// one KV head, a wavefront 32 of them, and all four share each tile of 64 keys in LDS
+// as FP16 integers: a thread loads 16 codes at a time two tiles ahead, converts them
+// once for the 128 columns and stores them double-buffered (one barrier a tile; 16-byte
+// chunks XOR-swizzled, K by 3 bits of the key that the 8 lanes of an access differ in, V
+// by the head dim).  S^T = K Q^T is then one FP16 product with q as it is.  What bounds
+// it: the softmax and its exponentials on the VALU, a third more than the matrix cores'
+// share.
+template <int HD>
+struct QrShape {
+    static constexpr int CH = HD / 8;             // 16-byte chunks of a K row
+    static constexpr int kK = 64 * HD * 2;        // bytes of a K tile, as many of V
+    static constexpr int kBuf = 2 * kK;
+    static constexpr int NI = HD / 64;            // pieces of 16 codes a thread and matrix
+    static constexpr int kShare = HD / 16 * 2 * 1024;   // O of a wavefront in a record
+    static constexpr int kRec = 4 * kShare + 128 * 8;   // a split's record: O, then m and l per column
+    static __device__ __forceinline__ int kswz(int key) { return (key & 3) | ((key >> 4) & 1) << 2; }
+};
+
+template <int HD>
+__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_rows_kernel(QaArgs a) {
+    using S = QrShape<HD>;
+    constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ uint32_t last;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
+
+    // ---- block -> (column tile, split, KV head): the last tiles first, they see the
+    // most keys
+    const int64_t b = (int64_t)gridDim.x - 1 - blockIdx.x;
+    const int g = (int)(b % a.n_kv);
+    const int64_t rest = b / a.n_kv;
+    const int s = (int)(rest % a.S);
+    const int64_t tile = rest / a.S;
+    int r = 0;
+    {
+        int hi = a.n_req;
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if ((int64_t)a.starts[mid] * G / 128 + mid <= tile) r = mid;
+            else hi = mid;
+        }
+    }
+    const int row0 = a.starts[r], n_new = a.starts[r + 1] - row0;
+    const int ti = (int)(tile - ((int64_t)row0 * G / 128 + r));
+    if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || ti < 0) return;
+    const int64_t ncol = (int64_t)n_new * G, c0 = 128 * (int64_t)ti;
+    if (c0 >= ncol || ncol <= 16) return;   // up to 16 columns are qa_kernel's
+    const int len = (int)min((int64_t)a.lens[r], (int64_t)a.max_blocks << a.pshift);
+    const int p0 = len - n_new;
+    auto low = [&](int p) { return a.window > 0 ? max(0, p - a.window + 1) : 0; };
+    const int t_first = (int)(c0 / G), t_last = (int)((min(c0 + 128, ncol) - 1) / G);
+    const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
+    const int n64 = max(0, (kend + 63) / 64 - k64);
+    const int ku = max(4, (n64 + a.S - 1) / a.S), T = max(1, (n64 + ku - 1) / ku);
+    if (s >= T) return;
+    const int tb = s * ku, te = min(n64, tb + ku);
+
+    // ---- this wavefront's columns: fragment f, lane l: column 16 f + l % 16 of its 32
+    const int64_t w0 = c0 + 32 * wave;
+    const bool works = w0 < ncol;
+    bool real[2];
+    int tok[2], head[2], plast[2], plow[2];
+    qa_h8 qf[2][NS];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+        const int64_t c = w0 + 16 * f + lc;
+        real[f] = c < ncol;
+        const int64_t cc = real[f] ? c : c0;
+        tok[f] = (int)(cc / G);
+        head[f] = g * G + (int)(cc % G);
+        plast[f] = real[f] ? p0 + tok[f] : -1;
+        plow[f] = low(p0 + tok[f]);
+        const uint16_t* const q = a.q + (int64_t)(row0 + tok[f]) * a.q_stride + (int64_t)head[f] * HD + 8 * lg;
+#pragma unroll
+        for (int d = 0; d < NS; ++d)
+            qf[f][d] = __builtin_bit_cast(qa_h8, (u4v)*reinterpret_cast<const qa_any16*>(q + 32 * d));
+    }
+    const int w_first = p0 + (int)(min(w0, ncol - 1) / G), w_last = p0 + (int)((min(w0 + 32, ncol) - 1) / G);
+
+    // ---- tiles through registers: piece i of a thread is 16 codes of key 16 grp + .. (K)
+    // and of head dim .. (V) of the 16 keys grp = thread / HD + i (256 / HD)
+    const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
+    const int last_block = max(0, (kend - 1) >> a.pshift);
+    const int in = threadIdx.x % HD, grp0 = __builtin_amdgcn_readfirstlane(threadIdx.x / HD);
+    const int kkey = in / (HD / 16), kunit = in % (HD / 16);   // K: key of the 16, piece of the row
+    u4v kx[NI], vx[NI];
+    // page ids a turn before the rows that they lead to, and those of the lane's 16 keys
+    int ids[NI], ps;
+    auto page_at = [&](int i, int grp) {
+        return *gptr<int32_t>(trow + min(((k64 + i) * 64 + 16 * grp) >> a.pshift, last_block));
+    };
+    auto look = [&](int i) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) ids[n] = page_at(i, grp0 + n * (256 / HD));
+        ps = page_at(i, lg);
+    };
+    auto issue = [&](int i) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int key = (k64 + i) * 64 + 16 * (grp0 + n * (256 / HD));
+            const int pg = ids[n] < 0 || ids[n] >= a.n_pages ? 0 : ids[n];
+            const int64_t hp = (int64_t)pg * a.n_kv + g;
+            kx[n] = *gptr<u4v>(a.Kc + (hp * page + (key & (page - 1)) + kkey) * HD + 16 * kunit);
+            vx[n] = *gptr<u4v>(a.Vc + (hp * HD + in) * page + (key & (page - 1)));
+        }
+    };
+    auto land = [&](int buf) {
+        unsigned char* const kt = smem + buf * S::kBuf;
+        unsigned char* const vt = kt + S::kK;
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int grp = grp0 + n * (256 / HD), key = 16 * grp + kkey;
+            u4v h[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t x0, x1, x2, x3;
+                codes_f16(kx[n][2 * e], x0, x1);
+                codes_f16(kx[n][2 * e + 1], x2, x3);
+                h[e] = u4v{x0, x1, x2, x3};
+            }
+            // the upper four pieces of a row store their second half first: the eight
+            // lanes of an access then touch distinct chunks
+            const int o = (kunit >> 2) & 1;
+            u4v* const krow = reinterpret_cast<u4v*>(kt + key * HD * 2);
+            krow[(2 * kunit + o) ^ S::kswz(key)] = o ? h[1] : h[0];
+            krow[(2 * kunit + 1 - o) ^ S::kswz(key)] = o ? h[0] : h[1];
+            u4v* const vrow = reinterpret_cast<u4v*>(vt + in * 128);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t x0, x1, x2, x3;
+                codes_f16(vx[n][2 * e], x0, x1);
+                codes_f16(vx[n][2 * e + 1], x2, x3);
+                vrow[(2 * grp + e) ^ (in & 7)] = u4v{x0, x1, x2, x3};
+            }
+        }
+    };
+    // the scales of the lane's 16 keys and whether their page is one
+    float sk, sv, sk2, sv2;
+    bool ok, ok2;
+    auto scales = [&] {
+        ok2 = ps >= 0 && ps < a.n_pages;
+        const int64_t hp = (int64_t)(ok2 ? ps : 0) * a.n_kv + g;
+        sk2 = *gptr<float>(a.ks + hp);
+        sv2 = *gptr<float>(a.vs + hp);
+    };
+
+    qa_f4 o[2][NJ];
+    float m[2], l[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+        m[f] = -INFINITY;
+        l[f] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[f][j] = qa_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float sl2 = 1.4426950408889634f / sqrtf((float)HD);
+    QaScale sc;
+    if (tb < te) {
+        look(tb);
+        issue(tb);
+        scales();
+        look(tb + 1);
+        land(0);
+        issue(tb + 1);
+    }
+    __syncthreads();
+    for (int i = tb; i < te; ++i) {
+        const int cur = (i - tb) & 1, key = (k64 + i) * 64;
+        const unsigned char* const kt = smem + cur * S::kBuf;
+        const unsigned char* const vt = kt + S::kK;
+        sk = sk2;
+        sv = sv2;
+        ok = ok2;
+        scales();   // of the next tile
+        look(i + 2);
+        if (works && key <= w_last && key + 63 >= low(w_first)) {
+            float y[2][4][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int kr = 16 * (lc >> 2) + 4 * t + (lc & 3);
+                qa_f4 acc[2] = {qa_f4{0.f, 0.f, 0.f, 0.f}, qa_f4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int d = 0; d < NS; ++d) {
+                    const qa_h8 kf = *reinterpret_cast<const qa_h8*>(kt + kr * HD * 2 + (((4 * d + lg) ^ S::kswz(kr)) << 4));
+#pragma unroll
+                    for (int f = 0; f < 2; ++f)
+                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[f][d], acc[f], 0, 0, 0);
+                }
+#pragma unroll
+                for (int f = 0; f < 2; ++f)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[f][t][e] = acc[f][e];
+            }
+            const bool whole = key + 63 <= w_first && key >= low(w_last) && __all(ok);
+            const int kk = key + 16 * lg;
+            sc.next(sv, [&](float al) {
+#pragma unroll
+                for (int f = 0; f < 2; ++f)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) o[f][j] *= al;
+            });
+            qa_h8 pb[2][2];
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+                qa_softmax(
+                    y[f], sl2 * sk, !whole,
+                    [&](int t, int e) { return !ok || kk + 4 * t + e > plast[f] || kk + 4 * t + e < plow[f]; }, sc, m[f],
+                    l[f], pb[f], [&](float al) {
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) o[f][j] *= al;
+                    });
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int d = 16 * j + lc;
+                    const qa_h8 vf = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ (d & 7)) << 4));
+#pragma unroll
+                    for (int f = 0; f < 2; ++f)
+                        o[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pb[f][u], o[f][j], 0, 0, 0);
+                }
+        }
+        if (i + 1 < te) {
+            land(cur ^ 1);
+            if (i + 2 < te) issue(i + 2);   // (a tile past the last has the last block's page)
+        }
+        __syncthreads();
+    }
+    const float unit = sc.unit();
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+        l[f] = quad_sum(l[f]);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[f][j] *= unit;
+    }
+    auto store = [&](int f, float sum) {
+        if (!real[f]) return;
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        uint16_t* const orow = a.out + (int64_t)(row0 + tok[f]) * a.out_stride + (int64_t)head[f] * HD + 4 * lg;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            u2v w;
+            w.x = (uint32_t)f2h(o[f][j][0] * inv) | ((uint32_t)f2h(o[f][j][1] * inv) << 16);
+            w.y = (uint32_t)f2h(o[f][j][2] * inv) | ((uint32_t)f2h(o[f][j][3] * inv) << 16);
+            *reinterpret_cast<qa_any8*>(orow + 16 * j) = w;
+        }
+    };
+    if (T == 1) {
+        if (works) {
+            store(0, l[0]);
+            store(1, l[1]);
+        }
+        return;
+    }
+
+    // ---- this split's record; the last workgroup adds them in split order, each
+    // wavefront its own columns
+    unsigned char* const grp = a.recs + (tile * a.n_kv + g) * (int64_t)a.S * S::kRec;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(grp, 0, 0x7fffffff, 0x00020000);
+    auto o_at = [&](int t, int f, int j) { return t * S::kRec + wave * S::kShare + (f * NJ + j) * 1024 + lane * 16; };
+    auto ml_at = [&](int t, int f) { return t * S::kRec + 4 * S::kShare + (32 * wave + 16 * f + lc) * 8; };
+    if (works) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4v, o[f][j]), rs, o_at(s, f, j), 0, kSc1);
+            if (lane < 16)
+                __builtin_amdgcn_raw_buffer_store_b64(u2v{__float_as_uint(m[f]), __float_as_uint(l[f])}, rs, ml_at(s, f), 0, kSc1);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint64_t* const word = a.cnt + tile * a.n_kv + g;
+    if (threadIdx.x == 0) {
+        last = tagged_arrive(word, a.tag) == (uint32_t)T ? 1u : 0u;
+        if (last) __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last || !works) return;
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+        float M = -INFINITY, L = 0.f;
+        for (int t = 0; t < T; ++t)
+            M = fmaxf(M, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, ml_at(t, f), 0, kSc1)));
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[f][j] = qa_f4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < T; ++t) {
+            const u2v ml = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rs, ml_at(t, f), 0, kSc1));
+            const float mt = __uint_as_float(ml.x), w = mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mt - M);
+            L += w * __uint_as_float(ml.y);
+            u4v ov[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                ov[j] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rs, o_at(t, f, j), 0, kSc1));
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[f][j] += __builtin_bit_cast(qa_f4, ov[j]) * w;
+        }
+        store(f, L);
+    }
+}
+
+// How a call is laid out.  Requests of up to 16 columns: a tile each in qa_kernel, their
+// keys over S workgroups; where longer ones are allowed for (max_new), those in
+// qa_rows_kernel, `tiles` of 128 columns at most, their keys over Sr workgroups.
 struct QaPlan {
-    int direct, S;
+    bool rows_too;
+    int S, Sr;
     int64_t tiles;
-    size_t cnt_bytes, rec_bytes;
+    size_t cnt_bytes, rec_bytes, rcnt_bytes, rrec_bytes;
+    size_t bytes() const { return cnt_bytes + rec_bytes + rcnt_bytes + rrec_bytes; }
 };
 
 QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len) {
     QaPlan p{};
-    const int G = n_q / n_kv, cus = num_cus();
-    p.direct = (int64_t)max_new * G <= 16;
-    p.tiles = p.direct ? n_req : (int64_t)rows * G / 16 + n_req;
-    // two workgroups a CU, and no more than 2048 keys to one where a tile is a
-    // request (ragged batches: one long conversation among short ones); at least
-    // 256 keys, a tile for each wavefront
-    const int64_t blocks = p.tiles * n_kv;
-    int64_t S = std::max<int64_t>(1, 2 * cus / blocks);
-    if (p.direct) S = std::max<int64_t>(S, (max_len + 2047) / 2048);
-    p.S = (int)std::min<int64_t>({S, (max_len + 255) / 256, 1024});
-    p.cnt_bytes = ((size_t)blocks * 8 + 255) / 256 * 256;
-    p.rec_bytes = p.S > 1 ? (size_t)blocks * p.S * (hd * 64 + 128) : 0;
+    const int64_t G = n_q / n_kv, cus = num_cus(), blocks = (int64_t)n_req * n_kv;
+    auto up = [](int64_t x) { return ((size_t)x + 255) / 256 * 256; };
+    // about a workgroup a CU, and no more than 4096 keys to one (ragged batches: a long
+    // conversation among short ones); 256 keys, a tile for each wavefront, at least.
+    // 16 requests of 750 to 1,500 keys, 16 / 8 heads of 128: 1 a CU 14.4 us, 2 a CU 16.5; one
+    // of 16,000, 32 / 8 heads: 20.1 and 30.0; 48 of 8,000 to 16,000: 4096 keys to one 209 us,
+    // 2048 223, 8192 226.
+    int64_t S = std::max<int64_t>({1, cus / blocks, ((int64_t)max_len + 4095) / 4096});
+    p.S = (int)std::min<int64_t>({S, ((int64_t)max_len + 255) / 256, kQaMaxSplits});
+    p.cnt_bytes = up(blocks * 8);
+    p.rec_bytes = p.S > 1 ? up(blocks * p.S * (hd * 64 + 128)) : 0;
+    p.rows_too = (int64_t)max_new * G > 16;
+    if (p.rows_too) {
+        p.tiles = (int64_t)rows * G / 128 + n_req;
+        const int64_t tb = p.tiles * n_kv;
+        p.Sr = (int)std::min<int64_t>({std::max<int64_t>(1, 2 * cus / tb), ((int64_t)max_len + 255) / 256, kQaMaxSplits});
+        p.rcnt_bytes = up(tb * 8);
+        p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * ((int64_t)hd * 512 + 1024)) : 0;
+    }
     return p;
 }
 
@@ -481,8 +833,7 @@ extern "C" {
 
 size_t bx_attention_paged_q8_workspace_bytes(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len) {
     if (rows <= 0 || n_req <= 0 || n_kv <= 0 || n_q <= 0 || n_q % n_kv || hd <= 0 || max_new <= 0 || max_len <= 0) return 0;
-    const QaPlan p = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
-    return p.cnt_bytes + p.rec_bytes;
+    return qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len).bytes();
 }
 
 int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, const int32_t* starts, const int32_t* lens,
@@ -500,32 +851,50 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     if ((int64_t)max_blocks * page > 0x7fffffff - 128)
         return fail(BX_EUNSUPPORTED, "attention_paged_q8: more than 2^31 - 129 tokens a request");
     const QaPlan p = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
-    if (ws_bytes < p.cnt_bytes + p.rec_bytes || (reinterpret_cast<uintptr_t>(ws) & 15))
+    if (ws_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(ws) & 15))
         return fail(BX_EINVAL, "attention_paged_q8: workspace too small or not 16-byte aligned");
-    if (p.tiles * n_kv * p.S > 0x7fffffff) return fail(BX_EUNSUPPORTED, "attention_paged_q8: too many rows and heads");
+    const int64_t blocks = (int64_t)n_req * n_kv * p.S, rblocks = p.tiles * n_kv * p.Sr;
+    if (blocks > 0x7fffffff || rblocks > 0x7fffffff)
+        return fail(BX_EUNSUPPORTED, "attention_paged_q8: too many rows and heads");
     QaArgs a{};
     a.q = q; a.q_stride = q_stride; a.rows = rows; a.starts = starts; a.lens = lens; a.n_req = n_req;
     a.table = table; a.max_blocks = max_blocks; a.pshift = __builtin_ctz((unsigned)page); a.n_pages = n_pages;
     a.Kc = Kc; a.Vc = Vc; a.ks = k_scale; a.vs = v_scale;
     a.n_kv = n_kv; a.G = n_q / n_kv; a.window = window; a.out = out; a.out_stride = out_stride;
-    a.direct = p.direct; a.S = p.S;
-    a.cnt = static_cast<uint64_t*>(ws);
-    a.recs = static_cast<unsigned char*>(ws) + p.cnt_bytes;
+    unsigned char* const w = static_cast<unsigned char*>(ws);
+    QaArgs ar = a;
+    a.S = p.S;
+    a.cnt = reinterpret_cast<uint64_t*>(w);
+    a.recs = w + p.cnt_bytes;
     a.tag = next_launch_tag();
-    const dim3 grid((unsigned)(p.tiles * n_kv * p.S));
-    const int lds = hd / 16 * 4096 + 512;
+    ar.S = p.Sr;
+    ar.cnt = reinterpret_cast<uint64_t*>(w + p.cnt_bytes + p.rec_bytes);
+    ar.recs = w + p.cnt_bytes + p.rec_bytes + p.rcnt_bytes;
+    ar.tag = next_launch_tag();
     hipStream_t st = as_stream(stream);
-    if (hd == 64) {
-        qa_kernel<64><<<grid, kQaThreads, lds, st>>>(a);
-    } else if (hd == 128) {
-        qa_kernel<128><<<grid, kQaThreads, lds, st>>>(a);
-    } else {
-        static std::atomic<uint64_t> allowed{0};
-        if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qa_kernel<256>), lds, "attention_paged_q8: LDS attribute"))
-            return rc;
-        qa_kernel<256><<<grid, kQaThreads, lds, st>>>(a);
-    }
-    return launch_check("attention_paged_q8");
+    auto run = [&](auto hdc) -> int {
+        constexpr int HD = decltype(hdc)::value, lds = HD / 16 * 4096 + 512, rlds = 2 * QrShape<HD>::kBuf;
+        if constexpr (lds > 64 * 1024) {
+            static std::atomic<uint64_t> allowed{0};
+            if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qa_kernel<HD>), lds, "attention_paged_q8: LDS attribute"))
+                return rc;
+        }
+        if (p.rows_too) {   // the long launch first
+            if constexpr (rlds > 64 * 1024) {
+                static std::atomic<uint64_t> allowed{0};
+                if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qa_rows_kernel<HD>), rlds,
+                                       "attention_paged_q8: LDS attribute"))
+                    return rc;
+            }
+            qa_rows_kernel<HD><<<(unsigned)rblocks, kQaThreads, rlds, st>>>(ar);
+            if (int rc = launch_check("attention_paged_q8 (rows)")) return rc;
+        }
+        qa_kernel<HD><<<(unsigned)blocks, kQaThreads, lds, st>>>(a);
+        return launch_check("attention_paged_q8");
+    };
+    if (hd == 64) return run(std::integral_constant<int, 64>{});
+    if (hd == 128) return run(std::integral_constant<int, 128>{});
+    return run(std::integral_constant<int, 256>{});
 }
 
 }  // extern "C"

@@ -384,8 +384,8 @@ int bx_kv_read_q8_f16(const int64_t* slots, int rows, int n_kv, int hd, int page
  * -> out (rows, n_q*hd), out_stride apart.  Query head h reads KV head h / (n_q /
  * n_kv), n_q / n_kv <= 16.  Rows from starts[n_req] on are left as they are; a row
  * that sees no key (more rows than keys; table entries that name no page hide
- * their keys) gives zeros.  max_new >= every request's rows (rows past max_new
- * may be left as they are) and max_len (about the longest request) shape the launch.
+ * their keys) gives zeros.  max_new >= every request's rows (a request
+ * with more may be left as it is) and max_len (about the longest request) shape the launch.
  * ws: bx_attention_paged_q8_workspace_bytes(...) bytes with the same arguments,
  * 16-byte aligned, zeroed once before its first use; calls sharing one must not
  * overlap. */
