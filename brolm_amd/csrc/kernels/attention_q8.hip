@@ -43,6 +43,7 @@ constexpr int kQaMaxGroup = 16;
 constexpr int kQaLazy = 8;      // the running maximum moves when exceeded by 2^8
 constexpr int kQaReserve = 7;   // 2^(8 + 7) < 65504
 constexpr int kQaMaxSplits = 256;   // their weights (16 columns) fit the LDS of the wavefronts' shares
+constexpr int64_t kQrRecBytes = 128 << 20;   // records of split chunks, at most
 constexpr int kQaMinExp = 6;    // least exponent field of the reference scale
 
 struct QaArgs {
@@ -238,15 +239,14 @@ struct QaTile {
 };
 
 template <int HD>
-__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs a) {
+__device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigned char* smem) {
     constexpr int NC = HD / 64, NJ = HD / 16;
-    extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
     // ---- block -> (request, split, KV head)
-    const int g = (int)(blockIdx.x % (unsigned)a.n_kv);
-    const int64_t rest = blockIdx.x / (unsigned)a.n_kv;
+    const int g = (int)(block % (unsigned)a.n_kv);
+    const int64_t rest = block / (unsigned)a.n_kv;
     const int s = (int)(rest % a.S);
     const int64_t tile = rest / a.S;
     const int r = (int)tile;
@@ -505,17 +505,15 @@ struct QrShape {
 };
 
 template <int HD>
-__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_rows_kernel(QaArgs a) {
+__device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, unsigned blocks, unsigned char* smem) {
     using S = QrShape<HD>;
     constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI;
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ uint32_t last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
     // ---- block -> (column tile, split, KV head): the last tiles first, they see the
     // most keys
-    const int64_t b = (int64_t)gridDim.x - 1 - blockIdx.x;
+    const int64_t b = (int64_t)blocks - 1 - block;
     const int g = (int)(b % a.n_kv);
     const int64_t rest = b / a.n_kv;
     const int s = (int)(rest % a.S);
@@ -761,12 +759,13 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_rows_kernel(Q
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     uint64_t* const word = a.cnt + tile * a.n_kv + g;
+    uint32_t* const last = reinterpret_cast<uint32_t*>(smem);   // (the tiles are done with)
     if (threadIdx.x == 0) {
-        last = tagged_arrive(word, a.tag) == (uint32_t)T ? 1u : 0u;
-        if (last) __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = tagged_arrive(word, a.tag) == (uint32_t)T ? 1u : 0u;
+        if (*last) __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!last || !works) return;
+    if (!*last || !works) return;
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
         float M = -INFINITY, L = 0.f;
@@ -787,6 +786,21 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_rows_kernel(Q
         }
         store(f, L);
     }
+}
+
+template <int HD>
+__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    qa_tile<HD>(a, blockIdx.x, smem);
+}
+
+// Both kinds of tiles in one launch, the long ones first: decode rows fill the CUs that
+// the chunks leave, or leave last.
+template <int HD>
+__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_both_kernel(QaArgs rows, QaArgs a, unsigned row_blocks) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    if (blockIdx.x < row_blocks) qa_rows_tile<HD>(rows, blockIdx.x, row_blocks, smem);
+    else qa_tile<HD>(a, blockIdx.x - row_blocks, smem);
 }
 
 // How a call is laid out.  Requests of up to 16 columns: a tile each in qa_kernel, their
@@ -815,11 +829,13 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     p.rec_bytes = p.S > 1 ? up(blocks * p.S * (hd * 64 + 128)) : 0;
     p.rows_too = (int64_t)max_new * G > 16;
     if (p.rows_too) {
+        // tiles at most; about as many as fill, unless every request leaves one in part
         p.tiles = (int64_t)rows * G / 128 + n_req;
-        const int64_t tb = p.tiles * n_kv;
-        p.Sr = (int)std::min<int64_t>({std::max<int64_t>(1, 2 * cus / tb), ((int64_t)max_len + 255) / 256, kQaMaxSplits});
+        const int64_t tb = p.tiles * n_kv, likely = std::max<int64_t>(1, (int64_t)rows * G / 128) * n_kv;
+        const int64_t rec = (int64_t)hd * 512 + 1024;
+        p.Sr = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / likely, ((int64_t)max_len + 511) / 512, kQrRecBytes / (tb * rec)}));
         p.rcnt_bytes = up(tb * 8);
-        p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * ((int64_t)hd * 512 + 1024)) : 0;
+        p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * rec) : 0;
     }
     return p;
 }
@@ -854,7 +870,7 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     if (ws_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(ws) & 15))
         return fail(BX_EINVAL, "attention_paged_q8: workspace too small or not 16-byte aligned");
     const int64_t blocks = (int64_t)n_req * n_kv * p.S, rblocks = p.tiles * n_kv * p.Sr;
-    if (blocks > 0x7fffffff || rblocks > 0x7fffffff)
+    if (blocks + rblocks > 0x7fffffff)
         return fail(BX_EUNSUPPORTED, "attention_paged_q8: too many rows and heads");
     QaArgs a{};
     a.q = q; a.q_stride = q_stride; a.rows = rows; a.starts = starts; a.lens = lens; a.n_req = n_req;
@@ -874,22 +890,19 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     hipStream_t st = as_stream(stream);
     auto run = [&](auto hdc) -> int {
         constexpr int HD = decltype(hdc)::value, lds = HD / 16 * 4096 + 512, rlds = 2 * QrShape<HD>::kBuf;
-        if constexpr (lds > 64 * 1024) {
+        auto allow = [&](std::atomic<uint64_t>& done, auto kernel, int bytes) {
+            return bytes <= 64 * 1024 ? BX_OK : allow_lds(done, reinterpret_cast<const void*>(kernel), bytes,
+                                                          "attention_paged_q8: LDS attribute");
+        };
+        if (p.rows_too) {
             static std::atomic<uint64_t> allowed{0};
-            if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qa_kernel<HD>), lds, "attention_paged_q8: LDS attribute"))
-                return rc;
+            if (int rc = allow(allowed, &qa_both_kernel<HD>, std::max(lds, rlds))) return rc;
+            qa_both_kernel<HD><<<(unsigned)(blocks + rblocks), kQaThreads, std::max(lds, rlds), st>>>(ar, a, (unsigned)rblocks);
+        } else {
+            static std::atomic<uint64_t> allowed{0};
+            if (int rc = allow(allowed, &qa_kernel<HD>, lds)) return rc;
+            qa_kernel<HD><<<(unsigned)blocks, kQaThreads, lds, st>>>(a);
         }
-        if (p.rows_too) {   // the long launch first
-            if constexpr (rlds > 64 * 1024) {
-                static std::atomic<uint64_t> allowed{0};
-                if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qa_rows_kernel<HD>), rlds,
-                                       "attention_paged_q8: LDS attribute"))
-                    return rc;
-            }
-            qa_rows_kernel<HD><<<(unsigned)rblocks, kQaThreads, rlds, st>>>(ar);
-            if (int rc = launch_check("attention_paged_q8 (rows)")) return rc;
-        }
-        qa_kernel<HD><<<(unsigned)blocks, kQaThreads, lds, st>>>(a);
         return launch_check("attention_paged_q8");
     };
     if (hd == 64) return run(std::integral_constant<int, 64>{});
