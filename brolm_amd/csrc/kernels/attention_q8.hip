@@ -113,57 +113,87 @@ struct QaScale {
     __device__ __forceinline__ float unit() const { return exp2_int(eref - 126 - kQaReserve); }
 };
 
-// One step of the softmax for 64 keys of a column: s[t][e] are the products of q and the
-// codes of key 4 t + e of the lane's 16, f their factor in base-2 units; hide(t, e) is
-// asked where `masked`.  The running maximum moves only when exceeded by 2^kQaLazy (rescale
-// then gets the factor of O).  The weights times the V scale come out as FP16 operands;
-// the scale enters in the exponent and leaves the sum as one factor (2^-60 in the place
-// of a zero, far below FP16).
-template <class H, class F>
-__device__ __forceinline__ void qa_softmax(float (&s)[4][4], float f, bool masked, H&& hide, const QaScale& sc, float& m,
-                                           float& l, qa_h8 (&pb)[2], F&& rescale) {
+// One step of the softmax for 64 keys of NF columns a lane: s[n][t][e] are the products of
+// q and the codes of key 4 t + e of the lane's 16, f their factor in base-2 units; hide(n,
+// t, e) is asked where `masked`.  The running maximum of a column moves only when
+// exceeded by 2^kQaLazy (rescale(al) then gets the factors of O).  The weights times the V
+// scale come out as FP16 operands; the scale enters in the exponent and leaves the sum as
+// one factor (2^-60 in the place of a zero, far below FP16).
+template <int NF, class H, class F>
+__device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const float (&cf)[NF], bool masked, H&& hide,
+                                           const QaScale& sc, float (&m)[NF], float (&l)[NF], qa_h8 (&pb)[NF][2],
+                                           F&& rescale) {
+    float f[NF], mx[NF], nm[NF];
+#pragma unroll
+    for (int n = 0; n < NF; ++n) f[n] = cf[n] * f0;
     if (masked) {
 #pragma unroll
+        for (int n = 0; n < NF; ++n) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][t][e] = hide(n, t, e) ? -INFINITY : s[n][t][e] * f[n];
+            f[n] = 1.f;
+        }
+    }
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < NF; ++n) {
+        mx[n] = s[n][0][0];
+#pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = hide(t, e) ? -INFINITY : s[t][e] * f;
-        f = 1.f;
+            for (int e = 0; e < 4; ++e) mx[n] = fmaxf(mx[n], s[n][t][e]);
+        mx[n] = quad_max(mx[n] * f[n]);
+        over |= mx[n] > m[n] + (float)kQaLazy;
     }
-    float mx = s[0][0];
+    if (__any(over)) {
+        float al[NF];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[t][e]);
-    mx = quad_max(mx * f);
-    if (__any(mx > m + (float)kQaLazy)) {
-        const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= al;
+        for (int n = 0; n < NF; ++n) {
+            const float mn = fmaxf(m[n], mx[n]);
+            al[n] = m[n] == mn ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
+            l[n] *= al[n];
+            m[n] = mn;
+        }
         rescale(al);
-        m = mn;
     }
-    const float nm = m == -INFINITY ? 0.f : -m;
-    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NF; ++n) nm[n] = m[n] == -INFINITY ? 0.f : -m[n];
     if (!sc.weird) {
-        const float r = fmaxf(sc.rv, 8.67361738e-19f), nr = nm + __builtin_amdgcn_logf(r);   // base-2 logarithm
+        const float r = fmaxf(sc.rv, 8.67361738e-19f), lr = __builtin_amdgcn_logf(r), ir = __builtin_amdgcn_rcpf(r);   // base 2
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int n = 0; n < NF; ++n) {
+            const float nr = nm[n] + lr;
+            float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], f, nr));
-                ls[e] += p;
-                pb[t / 2][4 * (t % 2) + e] = (_Float16)p;
-            }
-        l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), __builtin_amdgcn_rcpf(r), l);
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][e], f[n], nr));
+                    ls[e] += p;
+                    pb[n][t / 2][4 * (t % 2) + e] = (_Float16)p;
+                }
+            l[n] = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), ir, l[n]);
+        }
     } else {   // a hidden key weighs nothing whatever its page's scale
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int n = 0; n < NF; ++n)
+#pragma unroll 1
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], f, nm));
-                ls[e] += p;
-                pb[t / 2][4 * (t % 2) + e] = s[t][e] == -INFINITY ? (_Float16)0.f : (_Float16)(p * sc.rv);
-            }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                for (int e = 0; e < 4; ++e) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (q == t) x = s[n][q][e];
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f[n], nm[n]));
+                    l[n] += p;
+                    const _Float16 h = x == -INFINITY ? (_Float16)0.f : (_Float16)(p * sc.rv);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (q == t) pb[n][q / 2][4 * (q % 2) + e] = h;
+                }
     }
 }
 
@@ -311,7 +341,8 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     qa_f4 o[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) o[j] = qa_f4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    float mm[1] = {-INFINITY}, ll[1] = {0.f};
+    const float cfs[1] = {cf};
     QaScale sc;
     auto rescale = [&](float al) {
 #pragma unroll
@@ -321,7 +352,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     auto compute = [&](const QaTile<HD>& x, int i) {
         const int key = (k64 + i) * 64, kk = key + 16 * lg;
         // S: lane l, element e of y[t] holds key 16 (l / 16) + 4 t + e of column l % 16
-        float y[4][4];
+        float y[1][4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             qa_i4 h{0, 0, 0, 0}, w{0, 0, 0, 0};
@@ -331,15 +362,16 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
                 w = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qy.lo[c], w, 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[t][e] = (float)(h[e] * 256 + w[e]);
+            for (int e = 0; e < 4; ++e) y[0][t][e] = (float)(h[e] * 256 + w[e]);
             if (t == 1) __builtin_amdgcn_sched_barrier(0);   // two fragments' integer sums at a time
         }
         const bool whole = key + 63 <= p0 + t_first && key >= low(p0 + t_last) && __all(x.ok);
         sc.next(x.sv, rescale);
-        qa_h8 pb[2];
-        qa_softmax(
-            y, cf * x.sk, !whole,
-            [&](int t, int e) { return !x.ok || kk + 4 * t + e > plast || kk + 4 * t + e < plow; }, sc, m, l, pb, rescale);
+        qa_h8 pb[1][2];
+        qa_softmax<1>(
+            y, x.sk, cfs, !whole,
+            [&](int, int t, int e) { return !x.ok || kk + 4 * t + e > plast || kk + 4 * t + e < plow; }, sc, mm, ll, pb,
+            [&](const float (&al)[1]) { rescale(al[0]); });
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -348,7 +380,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
                 codes_f16(x.v[j][2 * u], e0, e1);
                 codes_f16(x.v[j][2 * u + 1], e2, e3);
                 const u4v w{e0, e1, e2, e3};
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qa_h8, w), pb[u], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qa_h8, w), pb[0][u], o[j], 0, 0, 0);
             }
     };
     // the page ids of the tile after next are requested before the next tile's rows: loads
@@ -374,7 +406,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
             ahead(x0, i + 4);
         }
     }
-    l = quad_sum(l);
+    const float m = mm[0], l = quad_sum(ll[0]);
     const float unit = sc.unit();
 
     // ---- the four wavefronts' shares -> head dims j = wave, wave + 4, .. of each
@@ -640,7 +672,7 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[f][j] = qa_f4{0.f, 0.f, 0.f, 0.f};
     }
-    const float sl2 = 1.4426950408889634f / sqrtf((float)HD);
+    const float sl2 = 1.4426950408889634f / sqrtf((float)HD), cfs[2] = {sl2, sl2};
     QaScale sc;
     if (tb < te) {
         look(tb);
@@ -687,15 +719,15 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
                     for (int j = 0; j < NJ; ++j) o[f][j] *= al;
             });
             qa_h8 pb[2][2];
+            qa_softmax<2>(
+                y, sk, cfs, !whole,
+                [&](int f, int t, int e) { return !ok || kk + 4 * t + e > plast[f] || kk + 4 * t + e < plow[f]; }, sc, m, l, pb,
+                [&](const float (&al)[2]) {
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
-                qa_softmax(
-                    y[f], sl2 * sk, !whole,
-                    [&](int t, int e) { return !ok || kk + 4 * t + e > plast[f] || kk + 4 * t + e < plow[f]; }, sc, m[f],
-                    l[f], pb[f], [&](float al) {
+                    for (int f = 0; f < 2; ++f)
 #pragma unroll
-                        for (int j = 0; j < NJ; ++j) o[f][j] *= al;
-                    });
+                        for (int j = 0; j < NJ; ++j) o[f][j] *= al[f];
+                });
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
