@@ -938,9 +938,10 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
         } else {
             // streaming loads where the keys may be more than the 256 MB cache holds (48
             // requests of 8,000 to 16,000 keys, 1.2 GB: 226 -> 209 us); smaller sets may
-            // still be there (16 of 750 to 1,500, 37 MB: 14.4 us, streaming 16.6)
-            const bool nt = (int64_t)n_req * max_len * n_kv * hd * 2 > (int64_t)256 << 20;
-            const auto kernel = nt ? qa_kernel<HD, true> : qa_kernel<HD, false>;
+            // still be there (16 of 750 to 1,500, 37 MB: 14.4 us, streaming 16.6), and heads of
+            // 256, one wavefront a SIMD, wait longer for them (234 us, streaming 243)
+            const bool nt = HD <= 128 && (int64_t)n_req * max_len * n_kv * hd * 2 > (int64_t)256 << 20;
+            const auto kernel = nt ? qa_kernel<HD, HD <= 128> : qa_kernel<HD, false>;
             static std::atomic<uint64_t> allowed[2];
             if (int rc = allow(allowed[nt], kernel, lds)) return rc;
             kernel<<<(unsigned)blocks, kQaThreads, lds, st>>>(a);

@@ -163,6 +163,39 @@ __device__ __forceinline__ void wave_sum_n(float (&v)[R]) {
     for (int r = 0; r < R; ++r) v[r] = lane63(v[r]);
 }
 
+// A value moved between lanes by DPP; lanes that receive none, and rows outside ROWS, get 0.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_of(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf, class T>
+__device__ __forceinline__ T dpp_of(T v) {   // 8 bytes: double, int64_t
+    const u2v w = __builtin_bit_cast(u2v, v);
+    const u2v y{dpp_of<CTRL, ROWS>(w.x), dpp_of<CTRL, ROWS>(w.y)};
+    return __builtin_bit_cast(T, y);
+}
+// Sum over the 16 lanes of a row, in every lane of it (quads, mirrored halves).
+template <class T>
+__device__ __forceinline__ T row16_sum(T v) {
+    v += dpp_of<0xB1>(v);
+    v += dpp_of<0x4E>(v);
+    v += dpp_of<0x141>(v);
+    v += dpp_of<0x140>(v);
+    return v;
+}
+// Inclusive prefix over the wavefront: shifts within rows, then the rows' last lanes
+// to the rows after them.
+template <class T>
+__device__ __forceinline__ T wave_prefix(T v) {
+    v += dpp_of<0x111>(v);
+    v += dpp_of<0x112>(v);
+    v += dpp_of<0x114>(v);
+    v += dpp_of<0x118>(v);
+    v += dpp_of<0x142, 0xA>(v);
+    v += dpp_of<0x143, 0xC>(v);
+    return v;
+}
+
 // Block-wide sum for blockDim.x == NT (multiple of 64); `red` is >= NT/64 floats of LDS.
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* red) {

@@ -24,7 +24,7 @@ namespace {
 // that arrives last, when all have read it.
 
 constexpr int kPlanThreads = 256;
-constexpr int kPlanRows = 1024;   // rows per workgroup
+constexpr int kPlanRows = 512;    // rows per workgroup
 
 struct PlanArgs {
     const int32_t *past, *delta;
@@ -38,26 +38,27 @@ struct PlanArgs {
     uint32_t tag;
 };
 
-// Exclusive prefix over the workgroup in thread order; *total gets the sum.
-__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* total) {
-    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int64_t inc = v;
+// Exclusive prefixes of three values over the workgroup in thread order, and their sums.
+__device__ __forceinline__ void plan_scan(int64_t (&v)[3], int64_t (&total)[3], int64_t (*red)[kPlanThreads / 64]) {
+    const int w = threadIdx.x >> 6;
+    int64_t inc[3];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(inc, o);
-        if (l >= o) inc += y;
+    for (int i = 0; i < 3; ++i) {
+        inc[i] = wave_prefix(v[i]);
+        if ((threadIdx.x & 63) == 63) red[i][w] = inc[i];
     }
     __syncthreads();
-    if (l == 63) red[w] = inc;
-    __syncthreads();
-    int64_t before = 0, sum = 0;
 #pragma unroll
-    for (int i = 0; i < kPlanThreads / 64; ++i) {
-        if (i < w) before += red[i];
-        sum += red[i];
+    for (int i = 0; i < 3; ++i) {
+        int64_t before = 0, sum = 0;
+#pragma unroll
+        for (int k = 0; k < kPlanThreads / 64; ++k) {
+            if (k < w) before += red[i][k];
+            sum += red[i][k];
+        }
+        total[i] = sum;
+        v[i] = before + inc[i] - v[i];
     }
-    *total = sum;
-    return before + inc - v;
 }
 
 // The last i in [0, n) with p[i] <= x (p ascending, p[0] = 0 <= x).
@@ -74,7 +75,7 @@ __device__ __forceinline__ int plan_find(const int32_t* p, int n, int x) {
 __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     // per request: first row, pages taken and pages given before it
     __shared__ int32_t s_row[kPlanMaxReq], s_take[kPlanMaxReq], s_give[kPlanMaxReq];
-    __shared__ int64_t red[kPlanThreads / 64];
+    __shared__ int64_t red[3][kPlanThreads / 64];
     __shared__ int s_bad;
     __shared__ uint32_t s_last;
     const int t = threadIdx.x, n = a.n_req, page = 1 << a.pshift;
@@ -97,10 +98,10 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
             give += ob > nb ? ob - nb : 0;
         }
     }
-    int64_t n_rows, n_take, n_give;
-    rows = plan_scan(rows, red, &n_rows);
-    take = plan_scan(take, red, &n_take);
-    give = plan_scan(give, red, &n_give);
+    int64_t pre[3] = {rows, take, give}, sum[3];
+    plan_scan(pre, sum, red);
+    rows = pre[0], take = pre[1], give = pre[2];
+    const int64_t n_rows = sum[0], n_take = sum[1], n_give = sum[2];
     if (head < 0 || tail < head || tail - head > a.n_pages || tail - head + n_give > a.n_pages) bad |= BX_KV_PLAN_BAD_RING;
     else if (n_take > tail - head) bad |= BX_KV_PLAN_NO_PAGES;
     if (n_rows > a.max_rows) bad |= BX_KV_PLAN_ROWS_FULL;

@@ -25,7 +25,6 @@
 // A 16-bit count wraps for more than 65,535 equal logits; the counts then add up
 // to less than the vocabulary, and the row is done again in pieces that cannot.
 #include <cmath>
-#include <type_traits>
 
 #include "common.h"
 
@@ -142,38 +141,6 @@ __device__ __forceinline__ void sr_count(int i, const u4v& x, bool all, int V, u
         if (j & 1) atomicAdd(reinterpret_cast<uint32_t*>(h + ((w >> 14) & 0x1fffcu)), __builtin_amdgcn_ubfe(w, 31, 1) * 65535u + 1u);
         else atomicAdd(reinterpret_cast<uint32_t*>(h + ((w << 2) & 0x1fffcu)), __builtin_amdgcn_ubfe(w, 15, 1) * 65535u + 1u);
     }
-}
-
-// A value moved between lanes by DPP; lanes that receive none, and rows outside ROWS, get 0.
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ uint32_t dpp_of(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ double dpp_of(double v) {
-    const u2v w = __builtin_bit_cast(u2v, v);
-    return __builtin_bit_cast(double, u2v{dpp_of<CTRL, ROWS>(w.x), dpp_of<CTRL, ROWS>(w.y)});
-}
-// Sum over the 16 lanes of a row, in every lane of it (quads, mirrored halves).
-template <class T>
-__device__ __forceinline__ T row16_sum(T v) {
-    v += dpp_of<0xB1>(v);
-    v += dpp_of<0x4E>(v);
-    v += dpp_of<0x141>(v);
-    v += dpp_of<0x140>(v);
-    return v;
-}
-// Inclusive prefix over the wavefront: shifts within rows, then the rows' last lanes
-// to the rows after them.
-template <class T>
-__device__ __forceinline__ T wave_prefix(T v) {
-    v += dpp_of<0x111>(v);
-    v += dpp_of<0x112>(v);
-    v += dpp_of<0x114>(v);
-    v += dpp_of<0x118>(v);
-    v += dpp_of<0x142, 0xA>(v);
-    v += dpp_of<0x143, 0xC>(v);
-    return v;
 }
 
 __device__ __forceinline__ int wave_max_i(int v) {
