@@ -193,9 +193,10 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
 // A wavefront's unit is 16 tokens of one head, in registers from the one load to
 // the store: of K a lane holds 8 head dims of hd / 32 tokens, of V 4 head dims of hd /
 // 16 consecutive tokens, which are consecutive bytes of the token-minor page.  Every
-// byte is read, requantized and written by one lane.  The four wavefronts of a
-// workgroup are the units of a page (and of 4 / (units) heads where a page has
-// fewer), which share its amax through LDS.
+// byte is read, requantized and written by one lane.  A run inside one unit (a decode
+// step's rows) is one wavefront's; for a longer one the four wavefronts of a workgroup are
+// the units of the page (and of 4 / (units) heads where a page has fewer) and share its
+// amax through LDS.
 
 typedef u4v __attribute__((aligned(2))) any16;
 typedef u2v __attribute__((aligned(2))) any8;
@@ -230,17 +231,19 @@ __device__ __forceinline__ uint32_t put_byte(uint32_t w, int i, int c) {
     return (w & ~(0xffu << (8 * i))) | ((uint32_t)(c & 0xff) << (8 * i));
 }
 
-// WHICH 0: K, 1: V; NCH units of 16 tokens a page.
-template <int HD, int WHICH, int NCH>
-__device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, int64_t slot, uint32_t* red) {
-    constexpr int HPW = NCH < 4 ? 4 / NCH : 1;   // heads a workgroup takes
-    constexpr int U = NCH > 4 ? NCH / 4 : 1;     // units a wavefront takes
+// WHICH 0: K, 1: V; NCH units of 16 tokens a page.  SOLO: the run lies inside one unit, head
+// hs of the workgroup's; else hs is not read.
+template <int HD, int WHICH, int NCH, bool SOLO>
+__device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, int64_t slot, int hs, uint32_t* red) {
+    constexpr int HPW = NCH < 4 ? 4 / NCH : 1;           // heads a workgroup takes
+    constexpr int U = NCH > 4 && !SOLO ? NCH / 4 : 1;    // units a wavefront takes
     constexpr int page = 16 * NCH;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hs = NCH < 4 ? wave / NCH : 0;
+    if (!SOLO) hs = NCH < 4 ? wave / NCH : 0;
     const int head = (int)blockIdx.y * HPW + hs;
     const bool there = head < a.n_kv;
     const int off = (int)(slot & (page - 1));
+    auto unit = [&](int u) { return SOLO ? off >> 4 : (NCH < 4 ? wave % NCH : wave) + 4 * u; };
     const int64_t hp = (slot >> a.pshift) * a.n_kv + (there ? head : 0);
     const int64_t st = a.stride[WHICH];
     // row of token tk of the page: x + tk st
@@ -270,7 +273,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
     bool has_new[U], part[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int c = (NCH < 4 ? wave % NCH : wave) + 4 * u, t0 = 16 * c;
+        const int c = unit(u), t0 = 16 * c;
         has_new[u] = there && t0 < off + n && t0 + 16 > off;
         part[u] = has_new[u] && WHICH == 1 && !(t0 + vt >= off && t0 + vt + VT <= off + n);
         // tokens outside the run read its nearest row and count as zero: loads without
@@ -300,7 +303,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
     uint32_t m = max(m2 & 0xffffu, m2 >> 16);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    if constexpr (NCH > 1) {
+    if constexpr (NCH > 1 && !SOLO) {
         if (lane == 0) red[wave] = m;
         __syncthreads();
         m = 0u;
@@ -314,10 +317,11 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
     const bool live = s > 0.f && s < INFINITY;   // else every code is 0
     const float div = live ? s : INFINITY, inv = live ? 1.0f / s : 0.f;
     const bool grew = off > 0 && new_bits != old_bits;
-    if ((NCH < 4 ? wave % NCH : wave) == 0 && lane == 0) *sp = s;
+    if ((SOLO || unit(0) == 0) && lane == 0) *sp = s;
+    const uint32_t mask = live ? 0xffffffffu : 0u;
     // the codes of four values, half h of each of four dwords
     auto code4 = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int h0, int h1, int h2, int h3) {
-        auto one = [&](uint32_t w, int h) { return (uint32_t)q8_code(h2f((uint16_t)(w >> (16 * h))), div, inv) & 0xffu; };
+        auto one = [&](uint32_t w, int h) { return (uint32_t)q8_code(h2f((uint16_t)((w & mask) >> (16 * h))), div, inv) & 0xffu; };
         return one(w0, h0) | (one(w1, h1) << 8) | (one(w2, h2) << 16) | (one(w3, h3) << 24);
     };
     // the earlier codes of one dword, the first of them token tk's and the others
@@ -330,10 +334,9 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
                 y = put_byte(y, b, live ? (int)rint((double)byte_of(y, b) * (double)s_old / (double)s) : 0);
         *p = y;
     };
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int c = (NCH < 4 ? wave % NCH : wave) + 4 * u, t0 = 16 * c;
-        if (grew && t0 < off) {
+    if (grew) {
+        auto move = [&](int c) {
+            const int t0 = 16 * c;
             if constexpr (WHICH == 0) {
 #pragma unroll 1
                 for (int j = 0; j < 2 * KL; ++j) {
@@ -346,9 +349,23 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
 #pragma unroll 1
                     for (int i = 0; i < VT / 4; ++i)
                         if (t0 + vt + 4 * i < off) move4(reinterpret_cast<uint32_t*>(v_piece(c, d)) + i, t0 + vt + 4 * i, 1);
-                if (part[u]) load_old(u, c);
             }
+        };
+        if constexpr (SOLO) {
+#pragma unroll 1
+            for (int c = 0; 16 * c < off; ++c) move(c);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (16 * unit(u) < off) move(unit(u));
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (part[u]) load_old(u, unit(u));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = unit(u), t0 = 16 * c;
         if (!has_new[u]) continue;
         if constexpr (WHICH == 0) {
 #pragma unroll
@@ -382,33 +399,54 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
     }
 }
 
-// Workgroup (window of rows, heads, K or V): the runs that start in its window, one
-// after the other.
+// Workgroup (window of rows, heads, K or V): the runs that start in its window.
 template <int HD, int NCH>
 __global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(AppendArgs a) {
     __shared__ uint32_t red[2][4];
     const int64_t row0 = (int64_t)blockIdx.x * a.window;
-    const int lane = threadIdx.x & 63;
-    constexpr int page = 16 * NCH;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int page = 16 * NCH, HPW = NCH < 4 ? 4 / NCH : 1;
     auto slot_at = [&](int64_t r) { return r >= 0 && r < a.rows ? a.slots[r] : -1; };
+    // lane l: row row0 + l; what starts a run in the window, and what continues none
     const int64_t r = row0 + lane, own = slot_at(r), prev = slot_at(r - 1);
-    const bool first = lane < a.window && own >= 0 && own < a.n_slots && ((own & (page - 1)) == 0 || own != prev + 1);
-    uint64_t todo = __ballot(first);
-    for (int k = 0; todo; k ^= 1) {   // red alternates: one barrier a run
+    const bool valid = own >= 0 && own < a.n_slots, next = valid && (own & (page - 1)) != 0 && own == prev + 1;
+    const uint64_t starts = __ballot(lane < a.window && valid && !next), stops = __ballot(!next);
+    // runs inside one unit: a wavefront each
+    uint64_t longer = 0;
+    int turn = 0;
+    for (uint64_t todo = starts; todo; todo &= todo - 1) {
         const int i = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        const int row = (int)(row0 + i);
-        const int64_t slot = a.slots[row];
-        const int left = page - (int)(slot & (page - 1));   // tokens to the page's end
-        int n = 0;
-        for (int q = 0; q < left; q += 64) {
-            const uint64_t same = __ballot(q + lane < left && slot_at((int64_t)row + q + lane) == slot + q + lane);
-            const int c = ~same ? __builtin_ctzll(~same) : 64;
-            n += c;
-            if (c < 64) break;
+        const uint64_t behind = i < 63 ? stops >> (i + 1) : 0;
+        const int64_t slot = __shfl(own, i);
+        const int n = behind ? __builtin_ctzll(behind) + 1 : 64;
+        if (n > 16 - (int)(slot & 15)) {
+            longer |= 1ull << i;
+            continue;
         }
-        if (blockIdx.z == 0) append_run<HD, 0, NCH>(a, row, n, slot, red[k]);
-        else append_run<HD, 1, NCH>(a, row, n, slot, red[k]);
+        // wavefront w: head w % HPW of the workgroup's, every (4 / HPW)th run
+        if (turn++ % (4 / HPW) != wave / HPW) continue;
+        if (blockIdx.z == 0) append_run<HD, 0, NCH, true>(a, (int)(row0 + i), n, slot, wave % HPW, nullptr);
+        else append_run<HD, 1, NCH, true>(a, (int)(row0 + i), n, slot, wave % HPW, nullptr);
+    }
+    if constexpr (NCH == 1) return;   // a page is one unit
+    // longer ones: all four, one after the other (red alternates: one barrier a run)
+    for (int k = 0; longer; k ^= 1) {
+        const int i = __builtin_ctzll(longer);
+        longer &= longer - 1;
+        const int row = (int)(row0 + i);
+        const int64_t slot = __shfl(own, i);
+        const int left = page - (int)(slot & (page - 1));   // tokens to the page's end
+        const uint64_t behind = i < 63 ? stops >> (i + 1) : 0;
+        int n = behind ? __builtin_ctzll(behind) + 1 : 64 - i;
+        if (!behind)
+            for (int q = n; q < left; q += 64) {
+                const uint64_t same = __ballot(q + lane < left && slot_at((int64_t)row + q + lane) == slot + q + lane);
+                const int c = ~same ? __builtin_ctzll(~same) : 64;
+                n += c;
+                if (c < 64) break;
+            }
+        if (blockIdx.z == 0) append_run<HD, 0, NCH, false>(a, row, n, slot, 0, red[k]);
+        else append_run<HD, 1, NCH, false>(a, row, n, slot, 0, red[k]);
     }
 }
 
@@ -564,9 +602,13 @@ int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, 
     a.rows = rows; a.n_kv = n_kv; a.pshift = __builtin_ctz((unsigned)page);
     a.n_slots = (int64_t)n_pages * page;
     a.slots = slots; a.codes[0] = Kc; a.codes[1] = Vc; a.scale[0] = k_scale; a.scale[1] = v_scale;
-    a.window = rows <= 1024 ? 1 : 16;
-    const unsigned windows = (unsigned)((rows + a.window - 1) / a.window);
+    // a row to a workgroup for few rows, as many as it has wavefronts for their heads where
+    // rows are many (decode rows are a wavefront each), 32 for prompts: three of 7,389 rows
+    // together, 8 heads of 128, pages of 64, 19.1 us (16 rows a workgroup 29.8, 4 55.3),
+    // 1,000 decode rows 30.2 us (a row a workgroup 37.4)
     const int per = page < 64 ? 64 / page : 1;   // heads a workgroup takes
+    a.window = rows <= 256 ? 1 : rows <= 2048 ? 4 / per : 32;
+    const unsigned windows = (unsigned)((rows + a.window - 1) / a.window);
     if ((n_kv + per - 1) / per > 65535) return fail(BX_EUNSUPPORTED, "kv_append_q8: too many heads");
     const dim3 grid(windows, (unsigned)((n_kv + per - 1) / per), 2);
     hipStream_t st = as_stream(stream);
