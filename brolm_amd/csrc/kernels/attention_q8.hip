@@ -47,6 +47,7 @@ constexpr int kQaLazy = 8;      // the running maximum moves when exceeded by 2^
 constexpr int kQaReserve = 7;   // 2^(8 + 7) < 65504
 constexpr int kQaMaxSplits = 256;   // their weights (16 columns) fit the LDS of the wavefronts' shares
 constexpr int64_t kQrRecBytes = 128 << 20;   // records of split chunks, at most
+constexpr int kQaWords = 32768;   // arrival counters of either kind of tile
 constexpr int kQaMinExp = 6;    // least exponent field of the reference scale
 
 struct QaArgs {
@@ -94,14 +95,17 @@ __device__ __forceinline__ float quad_sum(float v) {
 // The V scale of a lane's 16 keys relative to the reference, times 2^kQaReserve: the factor
 // that P carries into the FP16 operand.  The reference is a power of two at or above the
 // largest finite scale so far; where it moves, `rescale` gets the factor of the sums
-// made so far.  A NaN or an infinity takes no part in it (weird: some lane has one).
+// made so far.  A NaN or an infinity takes no part in it (weird: some lane has one), and
+// neither does a page of which the wavefront sees no key (seen): one behind a window may
+// have been given back and hold anything.
 struct QaScale {
     int eref = kQaMinExp;
     float rv;
     bool weird;
 
     template <class F>
-    __device__ __forceinline__ void next(float sv, F&& rescale) {
+    __device__ __forceinline__ void next(float sv, bool seen, F&& rescale) {
+        if (!seen) sv = 0.f;
         const bool fin = sv < INFINITY;
         weird = __any(!fin);
         int ev = fin ? (int)(__float_as_uint(sv) >> 23) : 0;
@@ -381,7 +385,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
             if (t == 1) __builtin_amdgcn_sched_barrier(0);   // two fragments' integer sums at a time
         }
         const bool whole = key + 63 <= p0 + t_first && key >= low(p0 + t_last) && __all(x.ok);
-        sc.next(x.sv, rescale);
+        sc.next(x.sv, x.ok && kk <= p0 + t_last && kk + 15 >= low(p0 + t_first), rescale);
         qa_h8 pb[1][4];
         qa_softmax<1, true>(
             y, x.sk, cfs, !whole,
@@ -729,7 +733,7 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
             }
             const bool whole = key + 63 <= w_first && key >= low(w_last) && __all(ok);
             const int kk = key + 16 * lg;
-            sc.next(sv, [&](float al) {
+            sc.next(sv, ok && kk <= w_last && kk + 15 >= low(w_first), [&](float al) {
 #pragma unroll
                 for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -859,8 +863,11 @@ struct QaPlan {
     bool rows_too;
     int S, Sr;
     int64_t tiles;
-    size_t cnt_bytes, rec_bytes, rcnt_bytes, rrec_bytes;
-    size_t bytes() const { return cnt_bytes + rec_bytes + rcnt_bytes + rrec_bytes; }
+    size_t rec_bytes, rrec_bytes;
+    // the counters have a place of their own whatever the call's shape, so that a workspace
+    // that serves different shapes keeps them at zero
+    static constexpr size_t kCounters = (size_t)2 * kQaWords * 8;
+    size_t bytes() const { return kCounters + rec_bytes + rrec_bytes; }
 };
 
 QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len) {
@@ -873,8 +880,7 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     // of 16,000, 32 / 8 heads: 20.1 and 30.0; 48 of 8,000 to 16,000: 4096 keys to one 209 us,
     // 2048 223, 8192 226.
     int64_t S = std::max<int64_t>({1, cus / blocks, ((int64_t)max_len + 4095) / 4096});
-    p.S = (int)std::min<int64_t>({S, ((int64_t)max_len + 255) / 256, kQaMaxSplits});
-    p.cnt_bytes = up(blocks * 8);
+    p.S = blocks > kQaWords ? 1 : (int)std::min<int64_t>({S, ((int64_t)max_len + 255) / 256, kQaMaxSplits});
     p.rec_bytes = p.S > 1 ? up(blocks * p.S * (hd * 64 + 128)) : 0;
     p.rows_too = (int64_t)max_new * G > 16;
     if (p.rows_too) {
@@ -882,8 +888,8 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         p.tiles = (int64_t)rows * G / 128 + n_req;
         const int64_t tb = p.tiles * n_kv, likely = std::max<int64_t>(1, (int64_t)rows * G / 128) * n_kv;
         const int64_t rec = (int64_t)hd * 512 + 1024;
-        p.Sr = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / likely, ((int64_t)max_len + 511) / 512, kQrRecBytes / (tb * rec)}));
-        p.rcnt_bytes = up(tb * 8);
+        p.Sr = (int)std::min<int64_t>({2 * cus / likely, ((int64_t)max_len + 511) / 512, kQrRecBytes / (tb * rec)});
+        if (p.Sr < 1 || tb > kQaWords) p.Sr = 1;
         p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * rec) : 0;
     }
     return p;
@@ -930,11 +936,11 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     QaArgs ar = a;
     a.S = p.S;
     a.cnt = reinterpret_cast<uint64_t*>(w);
-    a.recs = w + p.cnt_bytes;
+    a.recs = w + QaPlan::kCounters;
     a.tag = next_launch_tag();
     ar.S = p.Sr;
-    ar.cnt = reinterpret_cast<uint64_t*>(w + p.cnt_bytes + p.rec_bytes);
-    ar.recs = w + p.cnt_bytes + p.rec_bytes + p.rcnt_bytes;
+    ar.cnt = a.cnt + kQaWords;
+    ar.recs = a.recs + p.rec_bytes;
     ar.tag = next_launch_tag();
     hipStream_t st = as_stream(stream);
     auto run = [&](auto hdc) -> int {

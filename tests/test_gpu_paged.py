@@ -425,6 +425,58 @@ def test_attention_nan_stays_where_it_is_seen():
     release()
 
 
+@pytest.mark.parametrize("news", [[1, 1], [30, 1], [200, 3]])
+def test_attention_pages_behind_the_window_may_hold_anything(news):
+    """Pages that no row's window reaches have been given back: their codes and scales (NaN,
+    infinite, huge) change nothing, nor do those of tokens behind the last one."""
+    rng = np.random.default_rng(sum(news))
+    n_q, n_kv, hd, page, window, lens = 8, 2, 128, 16, 90, [700, 333]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    q = _f16(rng, int(starts[-1]), n_q, hd)
+    want, bound = pu.attention(cache, q, starts, lens, table, n_kv, window)
+    for r, (n, m) in enumerate(zip(lens, news)):
+        gone = table[r, :max(0, n - m - window + 1) // page]   # pages before the first row's window
+        for name, bad in (("ks", [np.nan, np.inf, 3e38]), ("vs", [3e38, np.nan, np.inf])):
+            cache[name][gone] = np.resize(np.array(bad, np.float32), (gone.size, n_kv))
+        last = table[r, (n - 1) // page]
+        cache["kc"][last][:, (n - 1) % page + 1:] = -128
+        cache["vc"][last][:, :, (n - 1) % page + 1:] = 127
+    c = Cache(cache)
+    out = c.attention(dev(q.view(np.uint16)).view(torch().float16).reshape(q.shape[0], -1), dev(starts),
+                      dev(np.array(lens, np.int32)), dev(table), n_q, max(news), max(lens), window)
+    got = host(out).astype(np.float64).reshape(q.shape)
+    assert (np.abs(got - want) <= bound + 2.0 ** -25).all()
+    release()
+
+
+def test_attention_one_workspace_for_many_shapes():
+    """Calls of different shapes in turn on one workspace, sized for the largest of them."""
+    t = torch()
+    rng = np.random.default_rng(21)
+    n_q, n_kv, hd, page = 8, 2, 64, 16
+    shapes = [([3000], [1], 0), ([40, 2000, 7], [40, 1, 3], 300), ([900] * 40, [1] * 40, 20), ([5000, 3], [20, 1], 0)]
+    sizes = [int(hip().bx_attention_paged_q8_workspace_bytes(sum(m), len(n), n_q, n_kv, hd, max(m), max(n))) for n, m, _ in shapes]
+    ws = t.zeros(max(sizes), dtype=t.uint8, device="cuda")
+    calls = []
+    for lens, news, window in shapes:
+        table, n_pages = _tables(rng, lens, page)
+        cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+        starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+        q = _f16(rng, int(starts[-1]), n_q, hd)
+        args = (dev(q.view(np.uint16)).view(t.float16).reshape(q.shape[0], -1), dev(starts), dev(np.array(lens, np.int32)),
+                dev(table), n_q, max(news), max(lens), window)
+        calls.append((Cache(cache), args, pu.attention(cache, q, starts, lens, table, n_kv, window)))
+    for turn in range(6):
+        for i in rng.permutation(len(calls)):
+            c, args, (want, bound) = calls[i]
+            got = host(c.attention(*args, ws=ws)).astype(np.float64).reshape(want.shape)
+            assert (np.abs(got - want) <= bound + 2.0 ** -25).all(), (turn, i)
+    assert not host(ws)[:512 * 1024].any()   # every counter back at zero
+    release()
+
+
 def test_attention_strided_rows_and_odd_addresses():
     rng = np.random.default_rng(9)
     n_q, n_kv, hd, page, lens, news = 8, 2, 128, 16, [100, 33], [20, 1]
