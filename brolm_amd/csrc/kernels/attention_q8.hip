@@ -83,13 +83,27 @@ __device__ __forceinline__ float exp2_int(int e) {   // 2^e, 0 below the normal 
     return e < -126 ? 0.f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23);
 }
 
-__device__ __forceinline__ float quad_max(float v) {   // over lanes l, l ^ 16, l ^ 32, l ^ 48
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+// op over lanes l, l ^ 16, l ^ 32, l ^ 48, in each of them: the two halves of the rows (of
+// the wavefront) that a lane swap hands out, without a trip through the LDS.
+template <class F>
+__device__ __forceinline__ uint32_t quad_of(uint32_t v, F&& op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op((uint32_t)b[0], (uint32_t)b[1]);
+}
+__device__ __forceinline__ float quad_max(float v) {
+    return __uint_as_float(quad_of(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
 }
 __device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    return __uint_as_float(quad_of(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+__device__ __forceinline__ uint32_t quad_max_u(uint32_t v) {
+    return quad_of(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
 // The V scale of a lane's 16 keys relative to the reference, times 2^kQaReserve: the factor
@@ -108,9 +122,7 @@ struct QaScale {
         if (!seen) sv = 0.f;
         const bool fin = sv < INFINITY;
         weird = __any(!fin);
-        int ev = fin ? (int)(__float_as_uint(sv) >> 23) : 0;
-        ev = max(ev, __shfl_xor(ev, 16));
-        ev = __builtin_amdgcn_readfirstlane(max(ev, __shfl_xor(ev, 32)));
+        const int ev = __builtin_amdgcn_readfirstlane((int)quad_max_u(fin ? __float_as_uint(sv) >> 23 : 0u));
         if (ev > eref) {
             rescale(exp2_int(eref - ev));
             eref = ev;
@@ -241,8 +253,7 @@ struct QaQuery {
                     m = max(m, max(a & 0xffffu, a >> 16));
                 }
             }
-        m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+        m = quad_max_u(m);
         const float amax = h2f((uint16_t)m);
         const bool fin = m < 0x7c00u;
         // the power of two that brings amax just below 32640 = 127 * 256 + 128
@@ -542,8 +553,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
 // one KV head, a wavefront 32 of them, and all four share each tile of 64 keys in LDS
 // as FP16 integers: a thread loads 16 codes at a time two tiles ahead, converts them
 // once for the 128 columns and stores them double-buffered (one barrier a tile; 16-byte
-// chunks XOR-swizzled, K by 3 bits of the key that the 8 lanes of an access differ in, V
-// by the head dim).  S^T = K Q^T is then one FP16 product with q as it is.  What bounds
+// chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with q as it is.  What bounds
 // it: the softmax and its exponentials on the VALU, a third more than the matrix cores'
 // share.
 template <int HD>
@@ -554,7 +564,13 @@ struct QrShape {
     static constexpr int NI = HD / 64;            // pieces of 16 codes a thread and matrix
     static constexpr int kShare = HD / 16 * 2 * 1024;   // O of a wavefront in a record
     static constexpr int kRec = 4 * kShare + 128 * 8;   // a split's record: O, then m and l per column
-    static __device__ __forceinline__ int kswz(int key) { return (key & 3) | ((key >> 4) & 1) << 2; }
+    // chunk c of key k sits at c ^ kswz(k), of head dim d at c ^ vswz(d): the 16 lanes that
+    // the LDS serves at once, 16 keys of a fragment or 16 head dims, then cover its 64
+    // banks, and so do the stores but those of K at 256
+    static __device__ __forceinline__ int kswz(int k) {
+        return CH == 8 ? ((k >> 4) & 3) << 1 | ((k >> 1) & 1) : ((k >> 4) & 3) << 2 | (k & 3);
+    }
+    static __device__ __forceinline__ int vswz(int d) { return (d >> 1) & 7; }
 };
 
 template <int HD>
@@ -650,27 +666,21 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
 #pragma unroll
         for (int n = 0; n < NI; ++n) {
             const int grp = grp0 + n * (256 / HD), key = 16 * grp + kkey;
-            u4v h[2];
+            u4v* const krow = reinterpret_cast<u4v*>(kt + key * HD * 2);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 uint32_t x0, x1, x2, x3;
                 codes_f16(kx[n][2 * e], x0, x1);
                 codes_f16(kx[n][2 * e + 1], x2, x3);
-                h[e] = u4v{x0, x1, x2, x3};
+                krow[(2 * kunit + e) ^ S::kswz(key)] = u4v{x0, x1, x2, x3};
             }
-            // the upper four pieces of a row store their second half first: the eight
-            // lanes of an access then touch distinct chunks
-            const int o = (kunit >> 2) & 1;
-            u4v* const krow = reinterpret_cast<u4v*>(kt + key * HD * 2);
-            krow[(2 * kunit + o) ^ S::kswz(key)] = o ? h[1] : h[0];
-            krow[(2 * kunit + 1 - o) ^ S::kswz(key)] = o ? h[0] : h[1];
             u4v* const vrow = reinterpret_cast<u4v*>(vt + in * 128);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 uint32_t x0, x1, x2, x3;
                 codes_f16(vx[n][2 * e], x0, x1);
                 codes_f16(vx[n][2 * e + 1], x2, x3);
-                vrow[(2 * grp + e) ^ (in & 7)] = u4v{x0, x1, x2, x3};
+                vrow[(2 * grp + e) ^ S::vswz(in)] = u4v{x0, x1, x2, x3};
             }
         }
     };
@@ -754,7 +764,7 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int d = 16 * j + lc;
-                    const qa_h8 vf = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ (d & 7)) << 4));
+                    const qa_h8 vf = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ S::vswz(d)) << 4));
 #pragma unroll
                     for (int f = 0; f < 2; ++f)
                         o[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pb[f][u], o[f][j], 0, 0, 0);
