@@ -346,7 +346,8 @@ int bx_f32_to_f16(const float* x, uint16_t* y, int64_t n, void* stream);
  * sits at ring[e mod n_pages].  Pages taken leave its head in the order of
  * requests, then blocks, and enter the table; pages given back (those that
  * none of the remaining tokens is in) join its tail in the same order.  Other
- * table entries stay as they are.  A new pool: ring[i] = i, ends = {0, n_pages}.
+ * table entries stay as they are.  A page belongs to one request at a time.  A new pool:
+ * ring[i] = i, ends = {0, n_pages}.
  * When *status is not 0, nothing else changes: lens = past, ends_out = ends_in,
  * every slot and position -1, every starts 0 (the step's other calls then do
  * nothing).  lens may be past and ends_out may be ends_in (the state in place).
