@@ -829,26 +829,37 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
     }
     __syncthreads();
     if (!*last || !works) return;
+    float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-        float M = -INFINITY, L = 0.f;
-        for (int t = 0; t < T; ++t)
-            M = fmaxf(M, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, ml_at(t, f), 0, kSc1)));
+        for (int f = 0; f < 2; ++f)
+            M[f] = fmaxf(M[f], __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, ml_at(t, f), 0, kSc1)));
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[f][j] = qa_f4{0.f, 0.f, 0.f, 0.f};
-        for (int t = 0; t < T; ++t) {
-            const u2v ml = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rs, ml_at(t, f), 0, kSc1));
-            const float mt = __uint_as_float(ml.x), w = mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mt - M);
-            L += w * __uint_as_float(ml.y);
-            u4v ov[NJ];
+#pragma unroll 1
+    for (int t = 0; t < T; ++t) {
+        u2v ml[2];
+        u4v ov[2][NJ];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            ml[f] = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rs, ml_at(t, f), 0, kSc1));
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
-                ov[j] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rs, o_at(t, f, j), 0, kSc1));
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) o[f][j] += __builtin_bit_cast(qa_f4, ov[j]) * w;
+                ov[f][j] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rs, o_at(t, f, j), 0, kSc1));
         }
-        store(f, L);
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const u2v x = ml[f];
+            const float mt = __uint_as_float(x.x), w = mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mt - M[f]);
+            L[f] += w * __uint_as_float(x.y);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[f][j] += __builtin_bit_cast(qa_f4, ov[f][j]) * w;
+        }
     }
+    store(0, L[0]);
+    store(1, L[1]);
 }
 
 template <int HD, bool NT>
