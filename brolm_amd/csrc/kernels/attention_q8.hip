@@ -46,7 +46,10 @@ constexpr int kQaMaxGroup = 16;
 constexpr int kQaLazy = 8;      // the running maximum moves when exceeded by 2^8
 constexpr int kQaReserve = 7;   // 2^(8 + 7) < 65504
 constexpr int kQaMaxSplits = 256;   // their weights (16 columns) fit the LDS of the wavefronts' shares
-constexpr int64_t kQrRecBytes = 128 << 20;   // records of split chunks, at most
+constexpr int64_t kQaRecBytes = 128 << 20;   // records of either kind of tile, at most
+constexpr int kQaNarrowReq = 256;    // requests whose narrow tiles a wavefront counts in four steps
+constexpr int kQaNarrowCols = 64;    // columns a request up to which narrow tiles serve any batch
+constexpr int64_t kQaNarrowWork = (int64_t)1 << 27;   // bytes of K that they read, for more columns
 constexpr int kQaWords = 32768;   // arrival counters of either kind of tile
 constexpr int kQaMinExp = 6;    // least exponent field of the reference scale
 
@@ -63,7 +66,7 @@ struct QaArgs {
     int n_kv, G, window;
     uint16_t* out;
     int64_t out_stride;
-    int S;
+    int narrow, S;
     uint64_t* cnt;
     unsigned char* recs;
     uint32_t tag;
@@ -300,21 +303,47 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
-    // ---- block -> (request, split, KV head)
+    // ---- block -> (tile of 16 columns, split, KV head)
     const int g = (int)(block % (unsigned)a.n_kv);
     const int64_t rest = block / (unsigned)a.n_kv;
     const int s = (int)(rest % a.S);
     const int64_t tile = rest / a.S;
-    const int r = (int)tile;
+    int r = (int)tile, c0 = 0;
+    if (a.narrow) {
+        // the tiles that have columns, numbered through: no empty block stands between two
+        // that work, or they would share their CUs and leave others idle
+        constexpr int N = kQaNarrowReq / 64;
+        int cnt[N], base = 0;
+        r = -1;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = min(64 * n + lane, a.n_req - 1), n_i = a.starts[i + 1] - a.starts[i];
+            cnt[n] = 64 * n + lane < a.n_req ? (int)(((int64_t)max(0, min(n_i, a.rows)) * G + 15) / 16) : 0;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int end = base + (int)wave_prefix((uint32_t)cnt[n]);
+            const uint64_t in = __ballot(end > tile && end - cnt[n] <= tile);
+            if (in) {
+                const int at = __builtin_ctzll(in);
+                r = 64 * n + at;
+                c0 = 16 * (int)(tile - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(cnt[n], at)));
+            }
+            base = __builtin_amdgcn_readlane(end, 63);
+        }
+        if (r < 0) return;
+    }
     const int row0 = a.starts[r], n_new = a.starts[r + 1] - row0;
-    if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || (int64_t)n_new * G > 16) return;
-    const int cols = n_new * G;
+    if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new) return;
+    const int64_t ncol = (int64_t)n_new * G;
+    if (!a.narrow && ncol > 16) return;
+    const int cols = (int)min((int64_t)16, ncol - c0);
     const int len = (int)min((int64_t)a.lens[r], (int64_t)a.max_blocks << a.pshift);
     // positions of the tile's first and last row, and of this lane's column
     const int p0 = len - n_new;
-    const int t_first = 0, t_last = n_new - 1;
+    const int t_first = c0 / G, t_last = (c0 + cols - 1) / G;
     const bool real = lc < cols;
-    const int col = real ? lc : 0, tok = col / G, head = g * G + col % G;
+    const int col = c0 + (real ? lc : 0), tok = col / G, head = g * G + col % G;
     auto low = [&](int p) { return a.window > 0 ? max(0, p - a.window + 1) : 0; };
     const int plast = real ? p0 + tok : -1, plow = low(p0 + tok);
     const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
@@ -549,7 +578,8 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     store(L);
 }
 
-// Prompt chunks: requests with more than 16 columns.  A workgroup takes 128 columns of
+// Prompt chunks: requests with more than 16 columns, where narrow tiles would cost more (the
+// plan below).  A workgroup takes 128 columns of
 // one KV head, a wavefront 32 of them, and all four share each tile of 64 keys in LDS
 // as FP16 integers: a thread loads 16 codes at a time two tiles ahead, converts them
 // once for the 128 columns and stores them double-buffered (one barrier a tile; 16-byte
@@ -878,12 +908,13 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_both_kernel(Q
 }
 
 // How a call is laid out.  Requests of up to 16 columns: a tile each in qa_kernel, their
-// keys over S workgroups; where longer ones are allowed for (max_new), those in
-// qa_rows_kernel, `tiles` of 128 columns at most, their keys over Sr workgroups.
+// keys over S workgroups; where longer ones are allowed for (max_new), those as several
+// such tiles (narrow), or in qa_rows_tile, `tiles` of 128 columns at most, their keys over
+// Sr workgroups.
 struct QaPlan {
-    bool rows_too;
+    bool rows_too, narrow;
     int S, Sr;
-    int64_t tiles;
+    int64_t tiles16, tiles;
     size_t rec_bytes, rrec_bytes;
     // the counters have a place of their own whatever the call's shape, so that a workspace
     // that serves different shapes keeps them at zero
@@ -893,23 +924,45 @@ struct QaPlan {
 
 QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len) {
     QaPlan p{};
-    const int64_t G = n_q / n_kv, cus = num_cus(), blocks = (int64_t)n_req * n_kv;
+    const int64_t G = n_q / n_kv, cus = num_cus(), cols16 = ((int64_t)rows * G + 15) / 16;
     auto up = [](int64_t x) { return ((size_t)x + 255) / 256 * 256; };
-    // about a workgroup a CU, and no more than 4096 keys to one (ragged batches: a long
-    // conversation among short ones); 256 keys, a tile for each wavefront, at least.
-    // 16 requests of 750 to 1,500 keys, 16 / 8 heads of 128: 1 a CU 14.4 us, 2 a CU 16.5; one
-    // of 16,000, 32 / 8 heads: 20.1 and 30.0; 48 of 8,000 to 16,000: 4096 keys to one 209 us,
-    // 2048 223, 8192 226.
-    int64_t S = std::max<int64_t>({1, cus / blocks, ((int64_t)max_len + 4095) / 4096});
-    p.S = blocks > kQaWords ? 1 : (int)std::min<int64_t>({S, ((int64_t)max_len + 255) / 256, kQaMaxSplits});
-    p.rec_bytes = p.S > 1 ? up(blocks * p.S * (hd * 64 + 128)) : 0;
+    // `tiles` of 16 columns at most, `likely` of them with any
+    auto small = [&](int64_t tiles, int64_t likely) {
+        // about a workgroup a CU, and no more than 4096 keys to one (ragged batches: a long
+        // conversation among short ones); 256 keys, a tile for each wavefront, at least.
+        // 16 requests of 750 to 1,500 keys, 16 / 8 heads of 128: 1 a CU 14.4 us, 2 a CU 16.5;
+        // one of 16,000, 32 / 8 heads: 20.1 and 30.0; 48 of 8,000 to 16,000: 4096 keys to one
+        // 209 us, 2048 223, 8192 226.
+        const int64_t rec = hd * 64 + 128;
+        const int64_t S = std::min<int64_t>({std::max<int64_t>({1, cus / (likely * n_kv), ((int64_t)max_len + 4095) / 4096}),
+                                             ((int64_t)max_len + 255) / 256, kQaMaxSplits, kQaRecBytes / (tiles * n_kv * rec)});
+        p.tiles16 = tiles;
+        p.S = tiles * n_kv > kQaWords ? 1 : (int)std::max<int64_t>(1, S);
+        p.rec_bytes = p.S > 1 ? up(tiles * n_kv * p.S * rec) : 0;
+    };
+    small(n_req, n_req);
     p.rows_too = (int64_t)max_new * G > 16;
+    if (p.rows_too && n_req <= kQaNarrowReq) {
+        // Narrow tiles for all rows: 31 us for a million keys of a tile of 16 columns where the
+        // chip is full, against 14 with all of a tile of 128, which is paid for whole; and
+        // where it is not full, more workgroups with less to do.  32 / 8 heads of 128, narrow
+        // against 128: 48 requests of 8,000 to 16,000 keys, 8 rows each 313 and 471 us, 12 411
+        // and 578; 16 of 750 to 1,500, 8 rows 17.0 and 29.4, 16 rows 25.3 and 35.8, 32 rows
+        // 42.2 and 41.7; one of 8,000, 64 rows 33.6 and 41.4; one prompt of 300, 16 / 8
+        // heads 10.8 and 16.8, of 1,000 27.2 and 26.8.
+        const int64_t likely = std::max((int64_t)n_req, cols16);
+        if ((int64_t)max_new * G <= kQaNarrowCols || likely * n_kv * max_len <= kQaNarrowWork / hd) {
+            small(n_req + (int64_t)rows * G / 16, likely);
+            p.narrow = true;
+            p.rows_too = false;
+        }
+    }
     if (p.rows_too) {
         // tiles at most; about as many as fill, unless every request leaves one in part
         p.tiles = (int64_t)rows * G / 128 + n_req;
         const int64_t tb = p.tiles * n_kv, likely = std::max<int64_t>(1, (int64_t)rows * G / 128) * n_kv;
         const int64_t rec = (int64_t)hd * 512 + 1024;
-        p.Sr = (int)std::min<int64_t>({2 * cus / likely, ((int64_t)max_len + 511) / 512, kQrRecBytes / (tb * rec)});
+        p.Sr = (int)std::min<int64_t>({2 * cus / likely, ((int64_t)max_len + 511) / 512, kQaRecBytes / (tb * rec)});
         if (p.Sr < 1 || tb > kQaWords) p.Sr = 1;
         p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * rec) : 0;
     }
@@ -945,7 +998,7 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     const QaPlan p = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
     if (ws_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(ws) & 15))
         return fail(BX_EINVAL, "attention_paged_q8: workspace too small or not 16-byte aligned");
-    const int64_t blocks = (int64_t)n_req * n_kv * p.S, rblocks = p.tiles * n_kv * p.Sr;
+    const int64_t blocks = p.tiles16 * n_kv * p.S, rblocks = p.tiles * n_kv * p.Sr;
     if (blocks + rblocks > 0x7fffffff)
         return fail(BX_EUNSUPPORTED, "attention_paged_q8: too many rows and heads");
     QaArgs a{};
@@ -955,6 +1008,7 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     a.n_kv = n_kv; a.G = n_q / n_kv; a.window = window; a.out = out; a.out_stride = out_stride;
     unsigned char* const w = static_cast<unsigned char*>(ws);
     QaArgs ar = a;
+    a.narrow = p.narrow;
     a.S = p.S;
     a.cnt = reinterpret_cast<uint64_t*>(w);
     a.recs = w + QaPlan::kCounters;
@@ -978,8 +1032,10 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
             // streaming loads where the keys may be more than the 256 MB cache holds (48
             // requests of 8,000 to 16,000 keys, 1.2 GB: 226 -> 209 us); smaller sets may
             // still be there (16 of 750 to 1,500, 37 MB: 14.4 us, streaming 16.6), and heads of
-            // 256, one wavefront a SIMD, wait longer for them (234 us, streaming 243)
-            const bool nt = HD <= 128 && (int64_t)n_req * max_len * n_kv * hd * 2 > (int64_t)256 << 20;
+            // 256, one wavefront a SIMD, wait longer for them (234 us, streaming 243); the narrow
+            // tiles of a request share its keys (48 of 8,000 to 16,000, 8 rows each: 313 us,
+            // streaming 406)
+            const bool nt = HD <= 128 && !p.narrow && (int64_t)n_req * max_len * n_kv * hd * 2 > (int64_t)256 << 20;
             const auto kernel = nt ? qa_kernel<HD, HD <= 128> : qa_kernel<HD, false>;
             static std::atomic<uint64_t> allowed[2];
             if (int rc = allow(allowed[nt], kernel, lds)) return rc;

@@ -388,8 +388,9 @@ int bx_kv_read_q8_f16(const int64_t* slots, int rows, int n_kv, int hd, int page
  * their keys) gives zeros.  max_new >= every request's rows (a request
  * with more may be left as it is) and max_len (about the longest request) shape the launch.
  * ws: bx_attention_paged_q8_workspace_bytes(...) bytes with the same arguments (the
- * largest of a program's shapes serves them all), 16-byte aligned, its first 512 KB zeroed
- * once before the first use; calls sharing one must not overlap. */
+ * largest of these over a program's shapes serves them all; a smaller shape may want more
+ * than a larger one), 16-byte aligned, its first 512 KB zeroed once before the first use;
+ * calls sharing one must not overlap. */
 size_t bx_attention_paged_q8_workspace_bytes(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len);
 int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, const int32_t* starts, const int32_t* lens,
                               int n_req, int max_new, int max_len, const int32_t* table, int max_blocks, int page,

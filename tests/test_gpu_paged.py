@@ -315,7 +315,7 @@ def test_append_strided_and_odd_addresses():
 
 # ----------------------------------------------------------------- attention
 
-def _attention_case(rng, lens, news, n_q, n_kv, hd, page, window=0, q_scale=1.0, pad=0):
+def _attention_case(rng, lens, news, n_q, n_kv, hd, page, window=0, q_scale=1.0, pad=0, max_new=None, max_len=None):
     table, n_pages = _tables(rng, lens, page)
     cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
     # scales of a cache of unit-variance keys and values, some pages far smaller
@@ -326,7 +326,7 @@ def _attention_case(rng, lens, news, n_q, n_kv, hd, page, window=0, q_scale=1.0,
     q = _f16(rng, rows, n_q, hd, scale=q_scale)
     c = Cache(cache)
     out = c.attention(f16_dev(q.astype(np.float32)).reshape(rows, -1).view(torch().float16), dev(starts),
-                      dev(np.array(lens, np.int32)), dev(table), n_q, max(news), max(lens), window)
+                      dev(np.array(lens, np.int32)), dev(table), n_q, max_new or max(news), max_len or max(lens), window)
     want, bound = pu.attention(cache, q, starts, lens, table, n_kv, window)
     got = host(out).astype(np.float64).reshape(rows, n_q, hd)
     n = int(starts[-1])
@@ -358,6 +358,39 @@ def test_attention_decode(n_q, n_kv, hd, page, lens):
 def test_attention_chunks(n_q, n_kv, hd, page, lens, news, window):
     rng = np.random.default_rng(sum(lens) + window)
     _attention_case(rng, lens, news, n_q, n_kv, hd, page, window, pad=3)
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd,page,lens,news", [
+    (8, 2, 128, 16, [200, 64, 1, 700], [50, 64, 1, 1]),
+    (8, 1, 64, 32, [130, 129], [130, 65]),
+    (6, 2, 256, 16, [100, 7], [33, 7]),
+    (3, 3, 128, 128, [400], [170]),
+    (16, 1, 128, 64, [90], [21]),
+    (4, 4, 64, 16, [257, 1, 80], [257, 1, 16]),
+    (4, 1, 128, 64, [2600, 1, 90], [300, 0, 4])])
+@pytest.mark.parametrize("window", [0, 37, 250])
+def test_attention_chunks_of_large_batches(n_q, n_kv, hd, page, lens, news, window):
+    """Tiles of 128 columns: bounds on rows and lengths that allow for far more work."""
+    rng = np.random.default_rng(sum(lens) + window + 1)
+    _attention_case(rng, lens, news, n_q, n_kv, hd, page, window, pad=3, max_new=max(news) + 65, max_len=1 << 21)
+
+
+@pytest.mark.parametrize("n_req,most", [(5, 40), (63, 9), (64, 9), (65, 9), (200, 5), (256, 5), (257, 5)])
+def test_attention_short_runs_of_many_requests(n_req, most):
+    """Zero to some rows a request, so that tiles begin and end anywhere; 257 requests are laid
+    out otherwise."""
+    rng = np.random.default_rng(n_req)
+    news = rng.integers(0, most + 1, n_req)
+    news[[0, -1]] = most
+    lens = news + rng.integers(0, 150, n_req)
+    _attention_case(rng, lens.tolist(), news.tolist(), 8, 1, 64, 16, window=int(n_req == 65) * 70, pad=1)
+
+
+def test_attention_single_tokens_under_a_loose_bound():
+    """max_new and max_len far above what comes."""
+    for max_new, max_len in ((7, 1 << 20), (64, 200), (64, 1 << 20)):
+        _attention_case(np.random.default_rng(max_new), [33, 150, 64], [1, 1, 1], 8, 2, 128, 32, pad=4, max_new=max_new,
+                        max_len=max_len)
 
 
 @pytest.mark.parametrize("news", [[1, 1], [30, 1]])
