@@ -319,10 +319,26 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
     const bool grew = off > 0 && new_bits != old_bits;
     if ((SOLO || unit(0) == 0) && lane == 0) *sp = s;
     const uint32_t mask = live ? 0xffffffffu : 0u;
-    // the codes of four values, half h of each of four dwords
-    auto code4 = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int h0, int h1, int h2, int h3) {
-        auto one = [&](uint32_t w, int h) { return (uint32_t)q8_code(h2f((uint16_t)((w & mask) >> (16 * h))), div, inv) & 0xffu; };
-        return one(w0, h0) | (one(w1, h1) << 8) | (one(w2, h2) << 16) | (one(w3, h3) << 24);
+    // the codes of four values, half h of each of four dwords: x inv + 1.5 2^23 has the rounded
+    // integer in its low byte.  x inv is x / s to 127 2^-24: right unless it lies within 2e-5
+    // of a half, which some lane's does one time in a hundred
+    auto code4 = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int h0, int h1, int h2, int h3) -> uint32_t {
+        auto val = [&](uint32_t w, int h) { return h2f((uint16_t)((w & mask) >> (16 * h))); };
+        const float x4[4] = {val(w0, h0), val(w1, h1), val(w2, h2), val(w3, h3)};
+        uint32_t u[4];
+        float far = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y = __builtin_fmaf(x4[i], inv, 12582912.f);
+            far = fmaxf(far, fabsf(__builtin_fmaf(x4[i], inv, -(y - 12582912.f))));
+            u[i] = __float_as_uint(y);
+        }
+        if (__any(far > 0.49998f)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = (uint32_t)q8_code(x4[i], div, inv);
+        }
+        const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+        return lo | hi;
     };
     // the earlier codes of one dword, the first of them token tk's and the others
     // `step` tokens apart, requantized in place
@@ -604,8 +620,8 @@ int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, 
     a.slots = slots; a.codes[0] = Kc; a.codes[1] = Vc; a.scale[0] = k_scale; a.scale[1] = v_scale;
     // a row to a workgroup for few rows, as many as it has wavefronts for their heads where
     // rows are many (decode rows are a wavefront each), 32 for prompts: three of 7,389 rows
-    // together, 8 heads of 128, pages of 64, 19.1 us (16 rows a workgroup 29.8, 4 55.3),
-    // 1,000 decode rows 30.2 us (a row a workgroup 37.4)
+    // together, 8 heads of 128, pages of 64, 15.6 us (16 rows a workgroup 24.0; 64 the same, but
+    // 18.4 for 16.6 with pages of 128), 1,000 decode rows 29.2 us (a row a workgroup 34.9)
     const int per = page < 64 ? 64 / page : 1;   // heads a workgroup takes
     a.window = rows <= 256 ? 1 : rows <= 2048 ? 4 / per : 32;
     const unsigned windows = (unsigned)((rows + a.window - 1) / a.window);

@@ -267,6 +267,34 @@ def test_append_rounds_ties_to_even():
     release()
 
 
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 128)])
+def test_append_values_next_to_halves(hd, page):
+    """Values whose quotient with the scale is as near to n + 1/2 as FP16 allows, on either side
+    of it, for scales that are powers of two (exact halves) and others."""
+    rng = np.random.default_rng(hd)
+    n_kv, pages = 2, 24
+    rows = pages * page
+    amax = np.where(rng.random((pages, 1, n_kv, 1)) < 0.5, 127.0 * 2.0 ** rng.integers(-15, 9, (pages, 1, n_kv, 1)),
+                    rng.uniform(1e-4, 6e4, (pages, 1, n_kv, 1))).astype(np.float16)
+    scale = (amax.astype(np.float32) / np.float32(127)).astype(np.float64)
+    x = ((rng.integers(-127, 127, (pages, page, n_kv, hd)) + 0.5) * scale).astype(np.float16)
+    step = rng.integers(-1, 2, x.shape)
+    x = np.where(step == 0, x, np.nextafter(x, np.where(step > 0, np.float16(np.inf), np.float16(-np.inf)).astype(np.float16)))
+    x = np.clip(x, -amax, amax).astype(np.float16)
+    x[:, 0, :, 0] = amax[:, 0, :, 0]
+    k = x.reshape(rows, n_kv, hd)
+    v = np.roll(k, 1, axis=2)
+    cache = pu.empty_cache(pages, n_kv, page, hd, rng)
+    slots = np.arange(rows, dtype=np.int64)
+    c = Cache(cache)
+    t = torch()
+    c.append(dev(k.view(np.uint16)).view(t.float16).reshape(rows, -1), dev(v.view(np.uint16)).view(t.float16).reshape(rows, -1),
+             dev(slots))
+    pu.append(cache, k, v, slots)
+    _same_cache(c.host(), cache, np.arange(pages))
+    release()
+
+
 def test_append_nan_and_infinity_stay_in_their_page_and_head():
     page, hd, n_kv = 16, 64, 3
     rng = np.random.default_rng(5)
