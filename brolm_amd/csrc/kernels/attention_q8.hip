@@ -125,8 +125,9 @@ struct QaScale {
         if (!seen) sv = 0.f;
         const bool fin = sv < INFINITY;
         weird = __any(!fin);
-        const int ev = __builtin_amdgcn_readfirstlane((int)quad_max_u(fin ? __float_as_uint(sv) >> 23 : 0u));
-        if (ev > eref) {
+        const uint32_t own = fin ? __float_as_uint(sv) >> 23 : 0u;
+        if (__any((int)own > eref)) {
+            const int ev = __builtin_amdgcn_readfirstlane((int)quad_max_u(own));
             rescale(exp2_int(eref - ev));
             eref = ev;
         }
@@ -146,9 +147,18 @@ template <int NF, bool SPLIT, class H, class F>
 __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const float (&cf)[NF], bool masked, H&& hide,
                                            const QaScale& sc, float (&m)[NF], float (&l)[NF], qa_h8 (&pb)[NF][SPLIT ? 4 : 2],
                                            F&& rescale) {
-    float f[NF], mx[NF], nm[NF];
+    // the exponents against the maximum so far: most tiles exceed it nowhere, and one that
+    // does moves them.  (The largest exponent costs half the instructions that the largest
+    // product does, which the compiler makes canonical first.)
+    float f[NF], nm[NF], nr[NF], mx[NF];
+    const float r = fmaxf(sc.rv, 8.67361738e-19f), lr = sc.weird ? 0.f : __builtin_amdgcn_logf(r);   // base 2
+    bool over = false;
 #pragma unroll
-    for (int n = 0; n < NF; ++n) f[n] = cf[n] * f0;
+    for (int n = 0; n < NF; ++n) {
+        f[n] = cf[n] * f0;
+        nm[n] = m[n] == -INFINITY ? 0.f : -m[n];
+        nr[n] = nm[n] + lr;
+    }
     if (masked) {
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
@@ -159,42 +169,44 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
             f[n] = 1.f;
         }
     }
-    bool over = false;
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
-        mx[n] = s[n][0][0];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[n] = fmaxf(mx[n], s[n][t][e]);
-        mx[n] = quad_max(mx[n] * f[n]);
-        over |= mx[n] > m[n] + (float)kQaLazy;
+            for (int e = 0; e < 4; ++e) {
+                s[n][t][e] = __builtin_fmaf(s[n][t][e], f[n], nr[n]);
+                mx[n] = t + e == 0 ? s[n][t][e] : fmaxf(mx[n], s[n][t][e]);
+            }
+        over |= mx[n] > (m[n] == -INFINITY ? -INFINITY : lr + (float)kQaLazy);
     }
     if (__any(over)) {
         float al[NF];
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
-            const float mn = fmaxf(m[n], mx[n]);
-            al[n] = m[n] == mn ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
+            const float mn = fmaxf(m[n], quad_max(mx[n] - nr[n]));
+            const float d = mn == m[n] ? 0.f : -mn - nm[n];
+            al[n] = mn == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
             l[n] *= al[n];
             m[n] = mn;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][t][e] += d;
         }
         rescale(al);
     }
-#pragma unroll
-    for (int n = 0; n < NF; ++n) nm[n] = m[n] == -INFINITY ? 0.f : -m[n];
     if (!sc.weird) {
-        const float r = fmaxf(sc.rv, 8.67361738e-19f), lr = __builtin_amdgcn_logf(r), ir = __builtin_amdgcn_rcpf(r);   // base 2
+        const float ir = __builtin_amdgcn_rcpf(r);
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
-            const float nr = nm[n] + lr;
-            float ls[4] = {0.f, 0.f, 0.f, 0.f};
+            float ls[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][e], f[n], nr));
-                    ls[e] += p;
+                    const float p = __builtin_amdgcn_exp2f(s[n][t][e]);
+                    ls[e] = t == 0 ? p : ls[e] + p;
                     const _Float16 h = (_Float16)p;
                     pb[n][t / 2][4 * (t % 2) + e] = h;
                     if constexpr (SPLIT) pb[n][2 + t / 2][4 * (t % 2) + e] = (_Float16)(p - (float)h);
@@ -212,7 +224,7 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         if (q == t) x = s[n][q][e];
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f[n], nm[n]));
+                    const float p = __builtin_amdgcn_exp2f(x);
                     l[n] += p;
                     const float pr = x == -INFINITY ? 0.f : p * sc.rv;
                     const _Float16 h = (_Float16)pr;
