@@ -618,7 +618,7 @@ struct QrShape {
 template <int HD>
 __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, unsigned blocks, unsigned char* smem) {
     using S = QrShape<HD>;
-    constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI;
+    constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI, KB = HD > 128 ? 1 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
@@ -766,18 +766,27 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
         scales();   // of the next tile
         look(i + 2);
         if (works && key <= w_last && key + 63 >= low(w_first)) {
+            // fragments from LDS a step ahead of the products that take them (heads of 256
+            // have no registers for K's)
             float y[2][4][4];
+            qa_h8 kf[KB][NS];
+            auto k_read = [&](int t) {
+                const int kr = 16 * (lc >> 2) + 4 * t + (lc & 3);
+#pragma unroll
+                for (int d = 0; d < NS; ++d)
+                    kf[t % KB][d] = *reinterpret_cast<const qa_h8*>(kt + kr * HD * 2 + (((4 * d + lg) ^ S::kswz(kr)) << 4));
+            };
+            if (KB > 1) k_read(0);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int kr = 16 * (lc >> 2) + 4 * t + (lc & 3);
+                if (t + KB - 1 < 4) k_read(t + KB - 1);
+                if constexpr (KB > 1) __builtin_amdgcn_sched_barrier(0);
                 qa_f4 acc[2] = {qa_f4{0.f, 0.f, 0.f, 0.f}, qa_f4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                for (int d = 0; d < NS; ++d) {
-                    const qa_h8 kf = *reinterpret_cast<const qa_h8*>(kt + kr * HD * 2 + (((4 * d + lg) ^ S::kswz(kr)) << 4));
+                for (int d = 0; d < NS; ++d)
 #pragma unroll
                     for (int f = 0; f < 2; ++f)
-                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[f][d], acc[f], 0, 0, 0);
-                }
+                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t % KB][d], qf[f][d], acc[f], 0, 0, 0);
 #pragma unroll
                 for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -801,16 +810,24 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) o[f][j] *= al[f];
                 });
+            qa_h8 vf[2][2];
+            auto v_read = [&](int j) {
+                const int d = 16 * j + lc;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+                for (int u = 0; u < 2; ++u)
+                    vf[j % 2][u] = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ S::vswz(d)) << 4));
+            };
+            v_read(0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int d = 16 * j + lc;
-                    const qa_h8 vf = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ S::vswz(d)) << 4));
+            for (int j = 0; j < NJ; ++j) {
+                if (j + 1 < NJ) v_read(j + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int f = 0; f < 2; ++f)
-                        o[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pb[f][u], o[f][j], 0, 0, 0);
-                }
+                        o[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j % 2][u], pb[f][u], o[f][j], 0, 0, 0);
+            }
         }
         if (i + 1 < te) {
             land(cur ^ 1);
