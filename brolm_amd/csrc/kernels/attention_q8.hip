@@ -26,6 +26,9 @@
 //
 // A column tile's keys are split over workgroups where there are few tiles; each
 // leaves a record (O, m, l), the last one to arrive adds them in split order.
+//
+// Single tokens are bound by their bytes: 48 requests of 8,000 to 16,000 keys, 8 KV heads of
+// 128, 5.6 TB/s of codes; one of 700 keys by latency (9.7 us: lengths, table, rows, the merge).
 #include <algorithm>
 
 #include "gemm_job.h"
@@ -591,13 +594,18 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
 }
 
 // Prompt chunks: requests with more than 16 columns, where narrow tiles would cost more (the
-// plan below).  A workgroup takes 128 columns of
-// one KV head, a wavefront 32 of them, and all four share each tile of 64 keys in LDS
-// as FP16 integers: a thread loads 16 codes at a time two tiles ahead, converts them
-// once for the 128 columns and stores them double-buffered (one barrier a tile; 16-byte
-// chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with q as it is.  What bounds
-// it: the softmax and its exponentials on the VALU, a third more than the matrix cores'
-// share.
+// plan below).  A workgroup takes 128 columns of one KV head, a wavefront 32 of them, and all
+// four share each tile of 64 keys in LDS as FP16 integers: a thread loads 16 codes at a time
+// two tiles ahead, converts them once for the 128 columns and stores them double-buffered
+// (one barrier a tile; 16-byte chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with
+// q as it is.
+// Two prompts of 2,047 rows, 32 / 8 heads of 128: 104 to 111 us, 600 to 640 TFLOP/s; 500 rows
+// at 16,000 keys 750.  What bounds it: two wavefronts a SIMD (240 registers, 64 KB of LDS a
+// workgroup), whose VALU work (exponents, exponentials, sums and the conversion of codes,
+// about 290 instructions a tile beside 64 matrix instructions) fills 58 % of the time, the
+// matrix cores 26 %, and a third of whose cycles wait, mostly at the tile's barrier.  Eight
+// wavefronts that share a tile convert half as much for 5 % and leave a batch half as many
+// workgroups; holding the next tile's conversion over the softmax spills (194 us).
 template <int HD>
 struct QrShape {
     static constexpr int CH = HD / 8;             // 16-byte chunks of a K row

@@ -22,6 +22,10 @@
 // keys one only: keys of one exponent are evenly spaced, so each weighs a constant
 // times the next.
 //
+// 16 rows of 151,936 ids: 31 us, 200 rows: 39.  What bounds it: one CU a row, whose LDS makes
+// 64 additions in about 16 cycles (15 us a row), the levels' exponentials (6 us), and the two
+// looks at the row.
+//
 // A 16-bit count wraps for more than 65,535 equal logits; the counts then add up
 // to less than the vocabulary, and the row is done again in pieces that cannot.
 #include <cmath>
