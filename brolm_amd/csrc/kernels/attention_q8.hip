@@ -75,6 +75,10 @@ struct QaArgs {
     uint32_t tag;
 };
 
+// The first key that the row at position p sees (p below 0 where there are more rows than
+// keys; the window may be anything up to 2^31 - 1).
+__device__ __forceinline__ int first_key(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
+
 // Four int8 codes as FP16 integers: 1024 + (c + 128) by byte placement, less 1152.
 __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
     const uint32_t u = w ^ 0x80808080u;
@@ -320,10 +324,9 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
 
     // ---- block -> (tile of 16 columns, split, KV head)
     const int g = (int)(block % (unsigned)a.n_kv);
-    const int64_t rest = block / (unsigned)a.n_kv;
-    const int s = (int)(rest % a.S);
-    const int64_t tile = rest / a.S;
-    int r = (int)tile, c0 = 0;
+    const unsigned rest = block / (unsigned)a.n_kv;
+    const int s = (int)(rest % (unsigned)a.S), tile = (int)(rest / (unsigned)a.S);
+    int r = tile, c0 = 0;
     if (a.narrow) {
         // the tiles that have columns, numbered through: no empty block stands between two
         // that work, or they would share their CUs and leave others idle
@@ -342,7 +345,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
             if (in) {
                 const int at = __builtin_ctzll(in);
                 r = 64 * n + at;
-                c0 = 16 * (int)(tile - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(cnt[n], at)));
+                c0 = 16 * (tile - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(cnt[n], at)));
             }
             base = __builtin_amdgcn_readlane(end, 63);
         }
@@ -353,13 +356,13 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     const int64_t ncol = (int64_t)n_new * G;
     if (!a.narrow && ncol > 16) return;
     const int cols = (int)min((int64_t)16, ncol - c0);
-    const int len = (int)min((int64_t)a.lens[r], (int64_t)a.max_blocks << a.pshift);
+    const int len = (int)min((int64_t)max(0, a.lens[r]), (int64_t)a.max_blocks << a.pshift);
     // positions of the tile's first and last row, and of this lane's column
     const int p0 = len - n_new;
     const int t_first = c0 / G, t_last = (c0 + cols - 1) / G;
     const bool real = lc < cols;
     const int col = c0 + (real ? lc : 0), tok = col / G, head = g * G + col % G;
-    auto low = [&](int p) { return a.window > 0 ? max(0, p - a.window + 1) : 0; };
+    auto low = [&](int p) { return first_key(p, a.window); };
     const int plast = real ? p0 + tok : -1, plow = low(p0 + tok);
     const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
     const int n64 = max(0, (kend + 63) / 64 - k64);
@@ -530,7 +533,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
 
     // ---- this split's record, then the sum of all by the last to arrive
     constexpr int kRec = NJ * 1024 + 128;   // O as the lanes hold it, m and l per column
-    unsigned char* const grp = a.recs + (tile * a.n_kv + g) * (int64_t)a.S * kRec;
+    unsigned char* const grp = a.recs + ((int64_t)tile * a.n_kv + g) * a.S * kRec;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(grp, 0, 0x7fffffff, 0x00020000);
     if (real) {
 #pragma unroll
@@ -632,11 +635,9 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
 
     // ---- block -> (column tile, split, KV head): the last tiles first, they see the
     // most keys
-    const int64_t b = (int64_t)blocks - 1 - block;
-    const int g = (int)(b % a.n_kv);
-    const int64_t rest = b / a.n_kv;
-    const int s = (int)(rest % a.S);
-    const int64_t tile = rest / a.S;
+    const unsigned b = blocks - 1 - block, rest = b / (unsigned)a.n_kv;
+    const int g = (int)(b % (unsigned)a.n_kv), s = (int)(rest % (unsigned)a.S);
+    const int64_t tile = rest / (unsigned)a.S;
     int r = 0;
     {
         int hi = a.n_req;
@@ -651,9 +652,9 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
     if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || ti < 0) return;
     const int64_t ncol = (int64_t)n_new * G, c0 = 128 * (int64_t)ti;
     if (c0 >= ncol || ncol <= 16) return;   // up to 16 columns are qa_kernel's
-    const int len = (int)min((int64_t)a.lens[r], (int64_t)a.max_blocks << a.pshift);
+    const int len = (int)min((int64_t)max(0, a.lens[r]), (int64_t)a.max_blocks << a.pshift);
     const int p0 = len - n_new;
-    auto low = [&](int p) { return a.window > 0 ? max(0, p - a.window + 1) : 0; };
+    auto low = [&](int p) { return first_key(p, a.window); };
     const int t_first = (int)(c0 / G), t_last = (int)((min(c0 + 128, ncol) - 1) / G);
     const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
     const int n64 = max(0, (kend + 63) / 64 - k64);
@@ -1030,8 +1031,8 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
     if (n_q / n_kv > kQaMaxGroup) return fail(BX_EUNSUPPORTED, "attention_paged_q8: GQA group larger than 16");
     if (q_stride < (int64_t)n_q * hd || out_stride < (int64_t)n_q * hd)
         return fail(BX_EINVAL, "attention_paged_q8: row stride below n_q * head_dim");
-    if ((int64_t)max_blocks * page > 0x7fffffff - 128)
-        return fail(BX_EUNSUPPORTED, "attention_paged_q8: more than 2^31 - 129 tokens a request");
+    if ((int64_t)max_blocks * page > 0x7fffffff - 4095)   // the tiles asked for ahead lie below 2^31 too
+        return fail(BX_EUNSUPPORTED, "attention_paged_q8: more than 2^31 - 4096 tokens a request");
     const QaPlan p = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
     if (ws_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(ws) & 15))
         return fail(BX_EINVAL, "attention_paged_q8: workspace too small or not 16-byte aligned");

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     // ---- the rows: position and slot; -1 behind the last one
     const int live = bad ? 0 : (int)n_rows;
     const int hm = bad ? 0 : (int)(head % a.n_pages), tm = bad ? 0 : (int)(tail % a.n_pages);
-    auto ring_at = [&](int base, int i) { return base + i < a.n_pages ? base + i : base + i - a.n_pages; };
+    auto ring_at = [&](int base, int i) { return base < a.n_pages - i ? base + i : base - (a.n_pages - i); };
     auto blocks_of = [&](int len) { return (int)(((int64_t)len + page - 1) >> a.pshift); };
     const int end = min(a.max_rows, ((int)blockIdx.x + 1) * kPlanRows);
     for (int i = (int)blockIdx.x * kPlanRows + t; i < end; i += kPlanThreads) {

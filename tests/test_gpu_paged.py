@@ -461,6 +461,29 @@ def test_attention_rows_without_keys():
     release()
 
 
+@pytest.mark.parametrize("max_new,max_len", [(4, 40), (40, 40), (100, 1 << 21)])
+def test_attention_windows_and_lengths_at_their_ends(max_new, max_len):
+    """The widest window with rows before the first key, and a length far below zero (no keys):
+    single-token tiles, several of them, tiles of 128 columns."""
+    rng = np.random.default_rng(max_new)
+    n_q, n_kv, hd, page, window = 4, 1, 64, 16, 2 ** 31 - 1
+    news, lens = [4, 2, 3, 1], [2, 40, -2 ** 31, 0]
+    if max_new > 4:
+        news[0] = max_new
+    table, n_pages = _tables(rng, [16, 40, 16, 16], page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    n = int(starts[-1])
+    q = _f16(rng, n, n_q, hd)
+    out = Cache(cache).attention(dev(q.view(np.uint16)).view(torch().float16).reshape(n, -1), dev(starts),
+                                 dev(np.array(lens, np.int32)), dev(table), n_q, max_new, max_len, window)
+    got = host(out).astype(np.float64).reshape(n, n_q, hd)
+    want, bound = pu.attention(cache, q, starts, np.maximum(lens, 0).tolist(), table, n_kv)
+    assert (np.abs(got - want) <= bound + 2.0 ** -25).all()
+    assert (got[:int(starts[1]) - 2] == 0).all() and (got[int(starts[2]):] == 0).all()
+    release()
+
+
 def test_attention_nan_stays_where_it_is_seen():
     """A NaN in a page's scale, in codes behind the last token, or in one query row
     reaches the rows that see it and no others."""
