@@ -366,7 +366,13 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     const int plast = real ? p0 + tok : -1, plow = low(p0 + tok);
     const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
     const int n64 = max(0, (kend + 63) / 64 - k64);
-    const int ku = max(4, (n64 + a.S - 1) / a.S), T = max(1, (n64 + ku - 1) / ku);
+    // Tiles to a workgroup: the S-th part at least.  A round of its four wavefronts takes 1.8 us
+    // and a record 0.33 us to join (heads of 128; the rounds of 256 twice that), so where that
+    // leaves few, the square root of all (one request of 8,000 keys 18.6 -> 14.9 us, 16,000 20.7
+    // -> 17.6); and up to 512 keys stay in one piece (300 keys 9.7 -> 8.5, 500 9.9 -> 8.7; 700
+    // 10.0 in three, 10.1 in one).
+    const int root = 4 * max(1, (int)((HD > 128 ? 0.18f : 0.25f) * __builtin_amdgcn_sqrtf((float)n64) + 0.5f));
+    const int ku = n64 <= 8 ? 8 : max(root, (n64 + a.S - 1) / a.S), T = max(1, (n64 + ku - 1) / ku);
     if (s >= T) return;
     const int tb = s * ku, te = min(n64, tb + ku);
 
@@ -962,14 +968,14 @@ struct QaPlan {
 
 QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len) {
     QaPlan p{};
-    const int64_t G = n_q / n_kv, cus = num_cus(), cols16 = ((int64_t)rows * G + 15) / 16;
+    const int64_t G = n_q / n_kv, cus = num_cus();
     auto up = [](int64_t x) { return ((size_t)x + 255) / 256 * 256; };
     // `tiles` of 16 columns at most, `likely` of them with any
     auto small = [&](int64_t tiles, int64_t likely) {
         // about a workgroup a CU, and no more than 4096 keys to one (ragged batches: a long
         // conversation among short ones); 256 keys, a tile for each wavefront, at least.
         // 16 requests of 750 to 1,500 keys, 16 / 8 heads of 128: 1 a CU 14.4 us, 2 a CU 16.5;
-        // one of 16,000, 32 / 8 heads: 20.1 and 30.0; 48 of 8,000 to 16,000: 4096 keys to one
+        // one of 16,000, 32 / 8 heads: 17.6 and 24.7; 48 of 8,000 to 16,000: 4096 keys to one
         // 209 us, 2048 223, 8192 226.
         const int64_t rec = hd * 64 + 128;
         const int64_t S = std::min<int64_t>({std::max<int64_t>({1, cus / (likely * n_kv), ((int64_t)max_len + 4095) / 4096}),
@@ -988,7 +994,9 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         // and 578; 16 of 750 to 1,500, 8 rows 17.0 and 29.4, 16 rows 25.3 and 35.8, 32 rows
         // 42.2 and 41.7; one of 8,000, 64 rows 33.6 and 41.4; one prompt of 300, 16 / 8
         // heads 10.8 and 16.8, of 1,000 27.2 and 26.8.
-        const int64_t likely = std::max((int64_t)n_req, cols16);
+        // requests with one row and, as many as the rest needs, with max_new
+        const int64_t more = std::max<int64_t>(0, (int64_t)rows - n_req), longer = std::min<int64_t>(n_req, (more + max_new - 2) / (max_new - 1));
+        const int64_t likely = n_req - longer + ((more + longer) * G + 15) / 16;
         if ((int64_t)max_new * G <= kQaNarrowCols || likely * n_kv * max_len <= kQaNarrowWork / hd) {
             small(n_req + (int64_t)rows * G / 16, likely);
             p.narrow = true;
