@@ -986,6 +986,10 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     };
     small(n_req, n_req);
     p.rows_too = (int64_t)max_new * G > 16;
+    // what the batch is taken to be: requests with one row and, as many as the rest needs,
+    // with max_new
+    const int64_t more = std::max<int64_t>(0, (int64_t)rows - n_req), most = std::max(2, max_new);
+    const int64_t longer = std::min<int64_t>(n_req, (more + most - 2) / (most - 1));
     if (p.rows_too && n_req <= kQaNarrowReq) {
         // Narrow tiles for all rows: 31 us for a million keys of a tile of 16 columns where the
         // chip is full, against 14 with all of a tile of 128, which is paid for whole; and
@@ -994,8 +998,6 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         // and 578; 16 of 750 to 1,500, 8 rows 17.0 and 29.4, 16 rows 25.3 and 35.8, 32 rows
         // 42.2 and 41.7; one of 8,000, 64 rows 33.6 and 41.4; one prompt of 300, 16 / 8
         // heads 10.8 and 16.8, of 1,000 27.2 and 26.8.
-        // requests with one row and, as many as the rest needs, with max_new
-        const int64_t more = std::max<int64_t>(0, (int64_t)rows - n_req), longer = std::min<int64_t>(n_req, (more + max_new - 2) / (max_new - 1));
         const int64_t likely = n_req - longer + ((more + longer) * G + 15) / 16;
         if ((int64_t)max_new * G <= kQaNarrowCols || likely * n_kv * max_len <= kQaNarrowWork / hd) {
             small(n_req + (int64_t)rows * G / 16, likely);
@@ -1004,11 +1006,32 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         }
     }
     if (p.rows_too) {
-        // tiles at most; about as many as fill, unless every request leaves one in part
+        // `tiles` at most.  As many workgroups as have room at once, two a CU (one with heads
+        // of 256), less one for every second CU where single tokens need some; a few more
+        // would run alone at the end.  32 / 8 heads of 128: 400 rows beside 7 single tokens at
+        // 6,000 keys 77 us in four parts, 97 in five (520 workgroups), 90 in three; 500 beside
+        // 39 at 4,000 89 in three, 104 in four; three of 126 to 200 rows and one token at 3,000
+        // 53 in three, 64 in four (544).  16 / 4 heads of 256, 500 rows at 4,000 90 in four,
+        // 122 in eight.
         p.tiles = (int64_t)rows * G / 128 + n_req;
-        const int64_t tb = p.tiles * n_kv, likely = std::max<int64_t>(1, (int64_t)rows * G / 128) * n_kv;
-        const int64_t rec = (int64_t)hd * 512 + 1024;
-        p.Sr = (int)std::min<int64_t>({2 * cus / likely, ((int64_t)max_len + 511) / 512, kQaRecBytes / (tb * rec)});
+        const int64_t tb = p.tiles * n_kv, rec = (int64_t)hd * 512 + 1024, slots = hd > 128 ? cus : 2 * cus;
+        const int64_t singles = hd > 128 ? 0 : std::min(cus / 2, (n_req - longer) * n_kv * p.S);
+        const int64_t likely = std::max<int64_t>(1, ((more + longer) * G + 127) / 128 + longer - 1) * n_kv;
+        int64_t Sr = std::max<int64_t>(1, std::min((slots - singles + likely / 2) / likely, slots / likely));
+        // More than one round where that is shorter by 15 %: a part takes its share of the
+        // keys and about four tiles' time to begin and to join (32 / 8 heads of 128, 1,500 rows
+        // at 8,000 keys: one round of 376 workgroups 281 us, 254 in parts; 1,100 beside 29
+        // single tokens at 12,000 447 and 358; 16 / 4 heads of 256, three chunks of 326 to 400
+        // rows at 2,000: 148 workgroups 142, 444 127).
+        auto time = [&](int64_t n) { return ((likely * n + slots - 1) / slots) * (max_len / 64.0 / n + 4.0); };
+        const double once = time(Sr);
+        double least = 0.85 * once;
+        for (int64_t n = slots / likely + 1; n <= 8; ++n)
+            if (time(n) < least) {
+                least = time(n);
+                Sr = n;
+            }
+        p.Sr = (int)std::min<int64_t>({Sr, ((int64_t)max_len + 511) / 512, kQaRecBytes / (tb * rec)});
         if (p.Sr < 1 || tb > kQaWords) p.Sr = 1;
         p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * rec) : 0;
     }
