@@ -608,11 +608,11 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
 // two tiles ahead, converts them once for the 128 columns and stores them double-buffered
 // (one barrier a tile; 16-byte chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with
 // q as it is.
-// Two prompts of 2,047 rows, 32 / 8 heads of 128: 104 to 111 us, 600 to 640 TFLOP/s; 500 rows
-// at 16,000 keys 750.  What bounds it: two wavefronts a SIMD (240 registers, 64 KB of LDS a
+// Two prompts of 2,047 rows, 32 / 8 heads of 128: 102 to 110 us, 600 to 655 TFLOP/s; 1,500 rows
+// at 12,000 keys 800.  What bounds it: two wavefronts a SIMD (240 registers, 64 KB of LDS a
 // workgroup), whose VALU work (exponents, exponentials, sums and the conversion of codes,
-// about 290 instructions a tile beside 64 matrix instructions) fills 58 % of the time, the
-// matrix cores 26 %, and a third of whose cycles wait, mostly at the tile's barrier.  Eight
+// about 290 instructions a tile beside 64 matrix instructions) fills 60 % of the time, the
+// matrix cores 27 %, and 27 % of whose cycles wait, mostly at the tile's barrier.  Eight
 // wavefronts that share a tile convert half as much for 5 % and leave a batch half as many
 // workgroups; holding the next tile's conversion over the softmax spills (194 us).
 template <int HD>
