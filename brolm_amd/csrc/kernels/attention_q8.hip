@@ -1017,7 +1017,8 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         const int64_t tb = p.tiles * n_kv, rec = (int64_t)hd * 512 + 1024, slots = hd > 128 ? cus : 2 * cus;
         const int64_t singles = hd > 128 ? 0 : std::min(cus / 2, (n_req - longer) * n_kv * p.S);
         const int64_t likely = std::max<int64_t>(1, ((more + longer) * G + 127) / 128 + longer - 1) * n_kv;
-        int64_t Sr = std::max<int64_t>(1, std::min((slots - singles + likely / 2) / likely, slots / likely));
+        const int64_t cap = std::max<int64_t>(1, std::min(((int64_t)max_len + 511) / 512, kQaRecBytes / (tb * rec)));
+        int64_t Sr = std::max<int64_t>(1, std::min({(slots - singles + likely / 2) / likely, slots / likely, cap}));
         // More than one round where that is shorter by 15 %: a part takes its share of the
         // keys and about four tiles' time to begin and to join (32 / 8 heads of 128, 1,500 rows
         // at 8,000 keys: one round of 376 workgroups 281 us, 254 in parts; 1,100 beside 29
@@ -1026,13 +1027,12 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         auto time = [&](int64_t n) { return ((likely * n + slots - 1) / slots) * (max_len / 64.0 / n + 4.0); };
         const double once = time(Sr);
         double least = 0.85 * once;
-        for (int64_t n = slots / likely + 1; n <= 8; ++n)
+        for (int64_t n = slots / likely + 1; n <= std::min<int64_t>(8, cap); ++n)
             if (time(n) < least) {
                 least = time(n);
                 Sr = n;
             }
-        p.Sr = (int)std::min<int64_t>({Sr, ((int64_t)max_len + 511) / 512, kQaRecBytes / (tb * rec)});
-        if (p.Sr < 1 || tb > kQaWords) p.Sr = 1;
+        p.Sr = tb > kQaWords ? 1 : (int)Sr;
         p.rrec_bytes = p.Sr > 1 ? up(tb * p.Sr * rec) : 0;
     }
     return p;
