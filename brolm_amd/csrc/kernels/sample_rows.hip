@@ -287,21 +287,31 @@ __global__ __launch_bounds__(kSrThreads) void sample_rows_kernel(SrArgs a) {
             __syncthreads();
         };
         block_sums(false);
-        // inclusive prefix over the blocks, thread t block t
+        // inclusive prefix over the blocks, thread t block t.  The sums form a tree, so a block
+        // without ids could differ from the block before it by a rounding; it takes that one's
+        // mass instead (a wavefront's lanes from the last with ids, and the wavefronts before it
+        // are added in one order), and a search for the first block past a goal ends in one
+        // that has ids.
         uint32_t n_in;
         double m_in;
         auto prefix = [&] {
-            n_in = wave_prefix(s.cnt[t]);
+            const uint32_t own = s.cnt[t];
+            n_in = wave_prefix(own);
             m_in = wave_prefix(s.mass[t]);
+            const uint64_t some = __ballot(own != 0u) & (~0ull >> (63 - lane));
+            const double last = __shfl(m_in, some ? 63 - __builtin_clzll(some) : 0);
+            m_in = some ? last : 0.0;
             if (lane == 63) {
                 s.red_n[wave] = n_in;
                 s.red_m[wave] = m_in;
             }
             __syncthreads();
+            double before = 0.0;
             for (int w = 0; w < wave; ++w) {
                 n_in += s.red_n[w];
-                m_in += s.red_m[w];
+                before += s.red_m[w];
             }
+            m_in += before;
         };
         prefix();
         uint32_t total = 0;
@@ -355,7 +365,8 @@ __global__ __launch_bounds__(kSrThreads) void sample_rows_kernel(SrArgs a) {
             return x;
         };
         auto last_lane = [](uint64_t mask) { return 63 - __builtin_clzll(mask); };
-        // the first block that passes (blocks behind it pass too), else the last one
+        // the first block that passes (blocks behind it pass too, but for a rounding), else the
+        // last one
         auto first_block = [&](auto&& pass) {
             const uint64_t far = __ballot(pass(16 * lane + 15));
             if (!far) return kSrBlocks - 1;
@@ -400,7 +411,8 @@ __global__ __launch_bounds__(kSrThreads) void sample_rows_kernel(SrArgs a) {
             SrLevels x = levels(bk);
             const uint64_t end = __ballot(x.c != 0u && x.before_n < n && n <= x.before_n + x.c);
             const double upto = x.before_m + (double)(n - x.before_n) * x.e;
-            const double goal = a.u[blockIdx.x] * __shfl(upto, end ? __builtin_ctzll(end) : 0);
+            // (not below 0: the blocks before the first with ids have a mass of 0)
+            const double goal = fmax(a.u[blockIdx.x] * __shfl(upto, end ? __builtin_ctzll(end) : 0), 0.0);
             const int bd = min(bk, first_block([&](int b) { return s.mass[b] > goal; }));
             if (bd != bk) x = levels(bd);
             const uint32_t c = x.before_n < n ? min(x.c, n - x.before_n) : 0u;   // kept ids of the level

@@ -161,3 +161,36 @@ def test_many_rows_and_replays():
         run()
         np.testing.assert_array_equal(host(out), got)
     release()
+
+
+def test_a_draw_between_two_levels_far_apart():
+    """Empty keys between the levels of a row: their running mass is that of the level before them
+    to the last bit, so that a draw next to it takes one of the row's ids."""
+    x = np.array([[7.76171875, 7.51171875, 7.26171875, 6.76171875]], np.float16)
+    got = _run(x, [0.360554575920105], None, None, None, [0.9655433869199928])
+    assert got[0] in (2, 3)
+
+
+def test_draws_around_every_border():
+    """u at each border between two ids of small rows, and up to 48 steps of FP64 to either
+    side: one of the two ids beside the border."""
+    rng = np.random.default_rng(8)
+    x, t, u, ids = [], [], [], []
+    for _ in range(120):
+        row = (rng.integers(-400, 400, 5) / 32).astype(np.float16)
+        temp = np.float32(rng.uniform(0.5, 6))
+        order = np.argsort(-row.astype(np.float64), kind="stable")
+        run = np.cumsum(np.exp((row[order].astype(np.float64) - float(row.max())) / float(temp)))
+        for j in range(4):
+            border = run[j] / run[-1]
+            if border > 1 - 2.0 ** -40:
+                continue
+            for k in range(-48, 49):
+                x.append(row)
+                t.append(temp)
+                u.append(border + k * np.spacing(border))
+                ids.append((order[j], order[j + 1]))
+    got = _run(np.array(x), t, None, None, None, u)
+    ids = np.array(ids)
+    bad = np.nonzero((got != ids[:, 0]) & (got != ids[:, 1]))[0]
+    assert bad.size == 0, [(x[i].tolist(), float(t[i]), u[i], int(got[i])) for i in bad[:4]]
