@@ -12,12 +12,12 @@
 //   softmax in FP32 (base 2, running maximum and sum per column); a tile's scales
 //         enter as one factor per 16 keys, which lie in one page;
 //   O^T += V^T P^T on v_mfma_f32_16x16x32_f16: V codes as FP16 integers, P times
-//         its page's scale of V.  That factor is taken relative to the largest
-//         scale so far, as a power of two with 2^7 in reserve, so P stays inside
-//         FP16 (below 2^15) and a page 2^20 times smaller than the largest still has
-//         11 bits.  A second product adds what P's rounding left: the output's error is then
-//         that of its own rounding (2.1e-4 relative; 3.1e-4 with one), for 1 % of the time,
-//         which goes with the bytes (48 requests of 8,000 to 16,000 keys 211 us, 208 with one).
+//         its page's scale of V.  The running maximum is that of score + log2(scale),
+//         so P stays inside FP16 (below 2^15) and what contributes 2^-21 of a column's
+//         largest part still has 11 bits.  A second product adds what P's rounding left:
+//         the output's error is then that of its own rounding (2.1e-4 relative; 3.1e-4
+//         with one), for 1 % of the time, which goes with the bytes (48 requests of 8,000
+//         to 16,000 keys 211 us, 208 with one).
 //         Prompt chunks, which the arithmetic bounds, leave it out.
 // The 16 keys that a lane holds of S^T are consecutive (fragment t takes the rows
 // 16 i + 4 t + j): P is an operand as it stands, and its V^T counterpart is one
@@ -47,14 +47,16 @@ typedef u2v __attribute__((aligned(2))) qa_any8;
 constexpr int kQaThreads = 256;
 constexpr int kQaMaxGroup = 16;
 constexpr int kQaLazy = 8;      // the running maximum moves when exceeded by 2^8
-constexpr int kQaReserve = 7;   // 2^(8 + 7) < 65504
+constexpr int kQaReserve = 7;   // P is 2^7 at that maximum; 2^(8 + 7) < 65504
+// V scales as P carries them: weights divided by one add up inside FP32.  127 times the least
+// is 0 in FP16, the most is infinite.
+constexpr float kQaLeastScale = 0x1p-64f, kQaMostScale = 0x1p64f;
 constexpr int kQaMaxSplits = 256;   // their weights (16 columns) fit the LDS of the wavefronts' shares
 constexpr int64_t kQaRecBytes = 128 << 20;   // records of either kind of tile, at most
 constexpr int kQaNarrowReq = 256;    // requests whose narrow tiles a wavefront counts in four steps
 constexpr int kQaNarrowCols = 64;    // columns a request up to which narrow tiles serve any batch
 constexpr int64_t kQaNarrowWork = (int64_t)1 << 27;   // bytes of K that they read, for more columns
 constexpr int kQaWords = 32768;   // arrival counters of either kind of tile
-constexpr int kQaMinExp = 6;    // least exponent field of the reference scale
 
 struct QaArgs {
     const uint16_t* q;
@@ -116,39 +118,28 @@ __device__ __forceinline__ uint32_t quad_max_u(uint32_t v) {
     return quad_of(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
-// The V scale of a lane's 16 keys relative to the reference, times 2^kQaReserve: the factor
-// that P carries into the FP16 operand.  The reference is a power of two at or above the
-// largest finite scale so far; where it moves, `rescale` gets the factor of the sums
-// made so far.  A NaN or an infinity takes no part in it (weird: some lane has one), and
-// neither does a page of which the wavefront sees no key (seen): one behind a window may
-// have been given back and hold anything.
+// The V scale that P carries for the lane's 16 keys.  A page of which the wavefront sees no key
+// (seen) may have been given back and hold anything; one with a NaN or an infinity that is seen
+// (weird: some lane has one) is multiplied apart.
 struct QaScale {
-    int eref = kQaMinExp;
-    float rv;
+    float sv, r;   // as it is; in P
     bool weird;
 
-    template <class F>
-    __device__ __forceinline__ void next(float sv, bool seen, F&& rescale) {
-        if (!seen) sv = 0.f;
+    __device__ __forceinline__ void next(float scale, bool seen) {
+        sv = seen ? scale : 1.f;
         const bool fin = sv < INFINITY;
         weird = __any(!fin);
-        const uint32_t own = fin ? __float_as_uint(sv) >> 23 : 0u;
-        if (__any((int)own > eref)) {
-            const int ev = __builtin_amdgcn_readfirstlane((int)quad_max_u(own));
-            rescale(exp2_int(eref - ev));
-            eref = ev;
-        }
-        rv = sv * exp2_int(126 + kQaReserve - eref);
+        r = fin ? fminf(fmaxf(sv, kQaLeastScale), kQaMostScale) : 1.f;
     }
-    __device__ __forceinline__ float unit() const { return exp2_int(eref - 126 - kQaReserve); }
 };
 
 // One step of the softmax for 64 keys of NF columns a lane: s[n][t][e] are the products of
 // q and the codes of key 4 t + e of the lane's 16, f their factor in base-2 units; hide(n,
-// t, e) is asked where `masked`.  The running maximum of a column moves only when
-// exceeded by 2^kQaLazy (rescale(al) then gets the factors of O).  The weights times the V
-// scale come out as FP16 operands; the scale enters in the exponent and leaves the sum as
-// one factor (2^-60 in the place of a zero, far below FP16).
+// t, e) is asked where `masked`.  m is the running maximum of score + log2(V scale), of each
+// column by itself: P, the weight times the V scale, is then near 2^kQaReserve where a column's
+// largest contributions are, whatever the scales of other pages or of those that only other
+// columns see, and as an FP16 operand loses bits only for what is 2^-21 of them.  It moves only
+// when exceeded by 2^kQaLazy (rescale(al) then gets the factors of O).  l is the sum of P / V scale.
 // SPLIT: pb[n][2 .. 3] gets what the rounding of pb[n][0 .. 1] left.
 template <int NF, bool SPLIT, class H, class F>
 __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const float (&cf)[NF], bool masked, H&& hide,
@@ -158,7 +149,7 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
     // does moves them.  (The largest exponent costs half the instructions that the largest
     // product does, which the compiler makes canonical first.)
     float f[NF], nm[NF], nr[NF], mx[NF];
-    const float r = fmaxf(sc.rv, 8.67361738e-19f), lr = sc.weird ? 0.f : __builtin_amdgcn_logf(r);   // base 2
+    const float lr = __builtin_amdgcn_logf(sc.r) + (float)kQaReserve;   // base 2
     bool over = false;
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
@@ -185,13 +176,13 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
                 s[n][t][e] = __builtin_fmaf(s[n][t][e], f[n], nr[n]);
                 mx[n] = t + e == 0 ? s[n][t][e] : fmaxf(mx[n], s[n][t][e]);
             }
-        over |= mx[n] > (m[n] == -INFINITY ? -INFINITY : lr + (float)kQaLazy);
+        over |= mx[n] > (m[n] == -INFINITY ? -INFINITY : (float)(kQaReserve + kQaLazy));
     }
     if (__any(over)) {
         float al[NF];
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
-            const float mn = fmaxf(m[n], quad_max(mx[n] - nr[n]));
+            const float mn = fmaxf(m[n], quad_max(mx[n] - nm[n] - (float)kQaReserve));
             const float d = mn == m[n] ? 0.f : -mn - nm[n];
             al[n] = mn == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
             l[n] *= al[n];
@@ -203,8 +194,8 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
         }
         rescale(al);
     }
+    const float ir = __builtin_amdgcn_rcpf(sc.r);
     if (!sc.weird) {
-        const float ir = __builtin_amdgcn_rcpf(r);
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
             float ls[4];
@@ -232,8 +223,8 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
                     for (int q = 0; q < 4; ++q)
                         if (q == t) x = s[n][q][e];
                     const float p = __builtin_amdgcn_exp2f(x);
-                    l[n] += p;
-                    const float pr = x == -INFINITY ? 0.f : p * sc.rv;
+                    l[n] = __builtin_fmaf(p, ir, l[n]);
+                    const float pr = sc.sv < INFINITY ? p : x == -INFINITY ? 0.f : p * sc.sv;
                     const _Float16 h = (_Float16)pr;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -449,7 +440,7 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
             if (t == 1) __builtin_amdgcn_sched_barrier(0);   // two fragments' integer sums at a time
         }
         const bool whole = key + 63 <= p0 + t_first && key >= low(p0 + t_last) && __all(x.ok);
-        sc.next(x.sv, x.ok && kk <= p0 + t_last && kk + 15 >= low(p0 + t_first), rescale);
+        sc.next(x.sv, x.ok && kk <= p0 + t_last && kk + 15 >= low(p0 + t_first));
         qa_h8 pb[1][4];
         qa_softmax<1, true>(
             y, x.sk, cfs, !whole,
@@ -492,13 +483,12 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
         }
     }
     const float m = mm[0], l = quad_sum(ll[0]);
-    const float unit = sc.unit();
 
     // ---- the four wavefronts' shares -> head dims j = wave, wave + 4, .. of each
     qa_f4* const so = reinterpret_cast<qa_f4*>(smem);            // [wave][j][lane]
     float* const sml = reinterpret_cast<float*>(so + 4 * NJ * 64);   // [wave][m, l][column]
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) so[(wave * NJ + j) * 64 + lane] = o[j] * unit;
+    for (int j = 0; j < NJ; ++j) so[(wave * NJ + j) * 64 + lane] = o[j];
     if (lane < 16) {
         sml[wave * 32 + lane] = m;
         sml[wave * 32 + 16 + lane] = l;
@@ -809,12 +799,7 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
             }
             const bool whole = key + 63 <= w_first && key >= low(w_last) && __all(ok);
             const int kk = key + 16 * lg;
-            sc.next(sv, ok && kk <= w_last && kk + 15 >= low(w_first), [&](float al) {
-#pragma unroll
-                for (int f = 0; f < 2; ++f)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) o[f][j] *= al;
-            });
+            sc.next(sv, ok && kk <= w_last && kk + 15 >= low(w_first));
             qa_h8 pb[2][2];
             qa_softmax<2, false>(
                 y, sk, cfs, !whole,
@@ -850,13 +835,8 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
         }
         __syncthreads();
     }
-    const float unit = sc.unit();
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-        l[f] = quad_sum(l[f]);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) o[f][j] *= unit;
-    }
+    for (int f = 0; f < 2; ++f) l[f] = quad_sum(l[f]);
     auto store = [&](int f, float sum) {
         if (!real[f]) return;
         const float inv = sum > 0.f ? 1.f / sum : 0.f;

@@ -1,0 +1,146 @@
+"""How exact the attention over the paged 8-bit cache is where its tiles mix things that
+a row's result must not depend on: pages of very different V scales, rows that
+see different pages, strong query channels, splits of a long context.  The reference is the
+softmax in 64 bits over the cache's values."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import paged_util as pu
+from gpu_util import dev, host, release, torch
+from test_gpu_paged import Cache, _tables
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(cache, q, starts, lens, table, n_kv, window=0, pair=True):
+    """(out, bound) in 64 bits.  pair: P in two FP16 parts (tiles of 16 columns), else one (tiles
+    of 128 columns).
+
+    The bound adds: the output's rounding, 2^-11 |o| + 2^-25; P's, 2^-21 A (its remainder's half
+    step) or 2^-11 A with A the mean of |v| under the weights, and below FP16's normal range 2^-25 of
+    a P whose largest is at least 2^7, for each of c keys, times a code of at most 127; a
+    score's error twice in the exponent: FP32 sums of hd products (hd 2^-24 sum |q k|), q to 2^-24
+    of its largest, and six FP32 roundings of an exponent of at most (|s| log2(e) + 64), whose
+    logarithm of a V scale adds 2^-18; FP32 sums of c products, (c + 64) 2^-23 A."""
+    n_pages, _, page, hd = cache["kc"].shape
+    rows, n_q = q.shape[:2]
+    group = n_q // n_kv
+    out, bound = np.zeros((rows, n_q, hd)), np.zeros((rows, n_q, hd))
+    for r in range(len(lens)):
+        n, m = int(lens[r]), int(starts[r + 1] - starts[r])
+        if n <= 0 or m <= 0:
+            continue
+        pages = table[r, :-(-n // page)]
+        k, v = pu.values(cache, pages)
+        sv = np.repeat(cache["vs"][pages].astype(np.float64), page, axis=0)[:n]   # (n, n_kv)
+        k, v = k[:n], v[:n]
+        for i in range(m):
+            p = n - m + i
+            lo = max(0, p - window + 1) if window else 0
+            if p < 0:
+                continue
+            row = int(starts[r]) + i
+            for g in range(n_kv):
+                qq = q[row, g * group:(g + 1) * group].astype(np.float64)
+                kk, vv, ss = k[lo:p + 1, g], v[lo:p + 1, g], sv[lo:p + 1, g]
+                s = qq @ kk.T / math.sqrt(hd)
+                w = np.exp(s - s.max(1, keepdims=True))
+                w /= w.sum(1, keepdims=True)
+                o, a = w @ vv, w @ np.abs(vv)
+                d = (hd * 2.0 ** -24 * (np.abs(qq) @ np.abs(kk).T) + 2.0 ** -24 * np.abs(qq).max() * np.abs(kk).sum(1)) / math.sqrt(hd)
+                d = d.max(1) + 6 * 2.0 ** -24 * (np.abs(s).max(1) + 64) + 2.0 ** -18
+                c = p + 1 - lo
+                rel = (2.0 ** -21 if pair else 2.0 ** -11) + np.expm1(2 * d) + (c + 64) * 2.0 ** -23
+                at = slice(g * group, (g + 1) * group)
+                out[row, at] = o
+                bound[row, at] = (2.0 ** -11 * np.abs(o) + 2.0 ** -25 + a * rel[:, None] +
+                                  c * 127 * 2.0 ** -32 * (w * ss).max(1)[:, None])
+    return out, bound
+
+
+def _run(cache, q, starts, lens, table, n_q, max_new, max_len, window=0):
+    rows = q.shape[0]
+    out = Cache(cache).attention(dev(q.view(np.uint16)).view(torch().float16).reshape(rows, -1),
+                                 dev(np.asarray(starts, np.int32)), dev(np.asarray(lens, np.int32)), dev(table), n_q,
+                                 max_new, max_len, window)
+    got = host(out).astype(np.float64).reshape(q.shape)
+    release()
+    return got
+
+
+def _within(got, want, bound, what):
+    worst = np.max(np.abs(got - want) / bound)
+    print(f"[precision] {what}: worst error / bound {worst:.3f}", flush=True)
+    assert np.isfinite(got).all() and worst <= 1, what
+
+
+def _grid(rng, *shape, scale=1.0):
+    """Queries in steps of 1/8: 16 bits hold them exactly."""
+    return (np.rint(np.clip(rng.standard_normal(shape) * scale, -15, 15) * 8) / 8).astype(np.float16)
+
+
+# rows, max_new, max_len: one tile of 16 columns, several of them, tiles of 128 columns
+KINDS = [("one", 4, 4, 50), ("narrow", 40, 40, 50), ("wide", 40, 105, 1 << 21)]
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind,news,max_new,max_len", KINDS)
+def test_rows_that_do_not_see_a_page_of_large_values(kind, news, max_new, max_len, hd):
+    """The last page holds values 2^26 times the others'; the rows before it, in the same tile of
+    columns, keep the bits of their own."""
+    rng = np.random.default_rng(hd + news)
+    n_q, n_kv, page, lens = 4, 2, 16, [50]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.02
+    cache["vs"][:] = 7e-6
+    cache["vs"][table[0, 3]] = 470.0
+    q = _grid(rng, news, n_q, hd)
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len)
+    want, bound = _attend(cache, q, [0, news], lens, table, n_kv, pair=kind != "wide")
+    _within(got, want, bound, kind)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("large", [0, 9, 40])
+@pytest.mark.parametrize("kind,news,max_new,max_len", [("one", 1, 1, 700), ("narrow", 40, 40, 700), ("wide", 40, 105, 1 << 21)])
+def test_weight_on_pages_of_small_values(kind, news, max_new, max_len, large, hd):
+    """A page of values 2^26 times the others' that the rows see and give no weight to."""
+    rng = np.random.default_rng(hd + news + large)
+    n_q, n_kv, page, lens = 4, 2, 16, [700]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.005
+    cache["vs"][:] = 7e-6
+    cache["vs"][table[0, large]] = 470.0
+    cache["ks"][table[0, large]] = 0.04
+    cache["kc"][table[0, large]] = -120        # q is positive: far below all other scores
+    q = np.abs(_grid(rng, news, n_q, hd, scale=3.0))
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len)
+    want, bound = _attend(cache, q, [0, news], lens, table, n_kv, pair=kind != "wide")
+    _within(got, want, bound, kind)
+
+
+@pytest.mark.parametrize("kind,news,max_new,max_len", [("one", 1, 1, 300), ("wide", 40, 105, 1 << 21)])
+def test_pages_of_zeros_and_extreme_scales(kind, news, max_new, max_len):
+    """V scales of zero (a page of zeros) and of 1e-36 beside ordinary ones: weights are shared
+    as the scores say, whatever the scale of what they weigh."""
+    rng = np.random.default_rng(news)
+    n_q, n_kv, hd, page, lens = 4, 2, 64, 32, [300]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.02
+    cache["vs"][:] = 0.02
+    cache["vs"][table[0, 1]] = 0.0
+    cache["vs"][table[0, 4], 0] = 1e-36
+    cache["vs"][table[0, 7], 1] = 1e-42
+    q = _grid(rng, news, n_q, hd)
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len)
+    want, bound = _attend(cache, q, [0, news], lens, table, n_kv, pair=kind != "wide")
+    _within(got, want, bound, kind)
+    cache["vs"][:] = 0.0   # only zeros in sight
+    assert (_run(cache, q, [0, news], lens, table, n_q, max_new, max_len) == 0).all()
