@@ -6,9 +6,10 @@
 // (row c / G, head c % G); a workgroup takes 16 columns of one KV head and walks
 // their keys in tiles of 64, one tile per wavefront at a time:
 //   S^T = K Q^T on v_mfma_i32_16x16x64_i8, the codes of K as they are stored: q is
-//         written as 256 hi + lo in two 8-bit parts times a power of two, both
-//         products are exact, and S = 256 S_hi + S_lo has q to 2^-15 of its largest
-//         element (components above 2^-5 of it exactly);
+//         written in three 8-bit parts times a power of two, whose products are exact,
+//         so S has q to 2^-23 of its largest element (components above 2^-11 of it
+//         exactly; with two parts, 2^-15, a channel 300 times the others cost 4e-3 of
+//         the output; the third takes 0.5 % of the time of a long decode step);
 //   softmax in FP32 (base 2, running maximum and sum per column); a tile's scales
 //         enter as one factor per 16 keys, which lie in one page;
 //   O^T += V^T P^T on v_mfma_f32_16x16x32_f16: V codes as FP16 integers, P times
@@ -240,8 +241,8 @@ __device__ __forceinline__ void qa_softmax(float (&s)[NF][4][4], float f0, const
 // holds column l % 16, head dims 64 c + 16 (l / 16) .. of part c.
 template <int HD>
 struct QaQuery {
-    qa_i4 hi[HD / 64], lo[HD / 64];
-    float scale;   // q = (256 hi + lo) scale; NaN where q holds one or an infinity
+    qa_i4 hi[HD / 64], mid[HD / 64], lo[HD / 64];
+    float scale;   // q = (65536 hi + 256 mid + lo) scale; NaN where q holds one or an infinity
     u4v w[HD / 64][2];
 
     // the loads apart from the arithmetic: the first tile is requested between them
@@ -269,26 +270,28 @@ struct QaQuery {
         m = quad_max_u(m);
         const float amax = h2f((uint16_t)m);
         const bool fin = m < 0x7c00u;
-        // the power of two that brings amax just below 32640 = 127 * 256 + 128
-        int k = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
-        if (amax * exp2_int(k) >= 32639.5f) --k;
+        // the power of two that brings amax below 127 * 65536 + 127 * 256 + 127, a whole number
+        int k = 22 - ((int)(__float_as_uint(amax) >> 23) - 127);
+        if (amax * exp2_int(k) > 8355711.f) --k;
         const float mul = fin && m > 0u ? exp2_int(k) : 0.f;
         scale = fin ? (m > 0u ? exp2_int(-k) : 0.f) : __uint_as_float(0x7fc00000u);
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                uint32_t h4 = 0u, l4 = 0u;
+                uint32_t h4 = 0u, m4 = 0u, l4 = 0u;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const int e = 4 * d + b;
                     const uint16_t x = (uint16_t)(w[c][e / 8][(e % 8) / 2] >> (16 * (e & 1)));
                     const int q = fin ? (int)rintf(h2f(x) * mul) : 0;
-                    const int h = (q + 128) >> 8;
+                    const int m = (q + 128) >> 8, h = (m + 128) >> 8;   // parts in [-128, 127]
                     h4 |= (uint32_t)(h & 0xff) << (8 * b);
-                    l4 |= (uint32_t)((q - 256 * h) & 0xff) << (8 * b);
+                    m4 |= (uint32_t)(m & 0xff) << (8 * b);
+                    l4 |= (uint32_t)(q & 0xff) << (8 * b);
                 }
                 hi[c][d] = (int)h4;
+                mid[c][d] = (int)m4;
                 lo[c][d] = (int)l4;
             }
     }
@@ -429,14 +432,16 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
         float y[1][4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            qa_i4 h{0, 0, 0, 0}, w{0, 0, 0, 0};
+            qa_i4 h{0, 0, 0, 0}, m{0, 0, 0, 0}, w{0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 h = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qy.hi[c], h, 0, 0, 0);
+                m = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qy.mid[c], m, 0, 0, 0);
                 w = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qy.lo[c], w, 0, 0, 0);
             }
+            // 256 h + m below 2^31 (256 * 256 * 128 * 129), the rest below 2^22
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[0][t][e] = (float)(h[e] * 256 + w[e]);
+            for (int e = 0; e < 4; ++e) y[0][t][e] = __builtin_fmaf((float)(h[e] * 256 + m[e]), 256.f, (float)w[e]);
             if (t == 1) __builtin_amdgcn_sched_barrier(0);   // two fragments' integer sums at a time
         }
         const bool whole = key + 63 <= p0 + t_first && key >= low(p0 + t_last) && __all(x.ok);

@@ -23,7 +23,7 @@ def _attend(cache, q, starts, lens, table, n_kv, window=0, pair=True):
     The bound adds: the output's rounding, 2^-11 |o| + 2^-25; P's, 2^-21 A (its remainder's half
     step) or 2^-11 A with A the mean of |v| under the weights, and below FP16's normal range 2^-25 of
     a P whose largest is at least 2^7, for each of c keys, times a code of at most 127; a
-    score's error twice in the exponent: FP32 sums of hd products (hd 2^-24 sum |q k|), q to 2^-24
+    score's error twice in the exponent: FP32 sums of hd products (hd 2^-24 sum |q k|), q to 2^-23
     of its largest, and six FP32 roundings of an exponent of at most (|s| log2(e) + 64), whose
     logarithm of a V scale adds 2^-18; FP32 sums of c products, (c + 64) 2^-23 A."""
     n_pages, _, page, hd = cache["kc"].shape
@@ -51,7 +51,7 @@ def _attend(cache, q, starts, lens, table, n_kv, window=0, pair=True):
                 w = np.exp(s - s.max(1, keepdims=True))
                 w /= w.sum(1, keepdims=True)
                 o, a = w @ vv, w @ np.abs(vv)
-                d = (hd * 2.0 ** -24 * (np.abs(qq) @ np.abs(kk).T) + 2.0 ** -24 * np.abs(qq).max() * np.abs(kk).sum(1)) / math.sqrt(hd)
+                d = (hd * 2.0 ** -24 * (np.abs(qq) @ np.abs(kk).T) + 2.0 ** -23 * np.abs(qq).max() * np.abs(kk).sum(1)) / math.sqrt(hd)
                 d = d.max(1) + 6 * 2.0 ** -24 * (np.abs(s).max(1) + 64) + 2.0 ** -18
                 c = p + 1 - lo
                 rel = (2.0 ** -21 if pair else 2.0 ** -11) + np.expm1(2 * d) + (c + 64) * 2.0 ** -23
@@ -144,3 +144,54 @@ def test_pages_of_zeros_and_extreme_scales(kind, news, max_new, max_len):
     _within(got, want, bound, kind)
     cache["vs"][:] = 0.0   # only zeros in sight
     assert (_run(cache, q, [0, news], lens, table, n_q, max_new, max_len) == 0).all()
+
+
+def _strong(rng, q, ratio):
+    """One channel of every head `ratio` times the others."""
+    q[..., 5] = np.where(rng.random(q.shape[:-1]) < 0.5, ratio, -ratio)
+    return q
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("ratio", [300, 3000])
+@pytest.mark.parametrize("kind,news,max_new,max_len", [("one", 2, 2, 9), ("narrow", 40, 40, 50), ("wide", 40, 105, 1 << 21)])
+def test_strong_query_channels(kind, news, max_new, max_len, ratio, hd):
+    """A channel that outweighs the others' size, where the keys have nothing: the scores are what
+    the other channels say."""
+    rng = np.random.default_rng(hd + ratio + news)
+    n_q, n_kv, page, lens = 4, 2, 16, [max(9, news)]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.01
+    cache["vs"][:] = 0.02
+    cache["kc"][..., 5] = 0
+    q = _strong(rng, rng.standard_normal((news, n_q, hd)), ratio).astype(np.float16)
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len)
+    want, bound = _attend(cache, q, [0, news], lens, table, n_kv, pair=kind != "wide")
+    _within(got, want, bound, kind)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("ratio", [0, 300])
+@pytest.mark.parametrize("kind,news,max_new,max_len", [("one", 1, 1, 2000), ("narrow", 32, 32, 2000), ("wide", 40, 105, 1 << 21)])
+def test_relative_error(kind, news, max_new, max_len, ratio, hd):
+    """The error's size over all outputs.  A rounding to FP16 is uniform over a step of at most
+    2^-10 of the value: 2^-11 / sqrt(3) = 2.82e-4 of it in the mean square, for the output, and once
+    more where P is one part (values of either sign: the errors add like the products).  All
+    other steps are below 1e-5."""
+    rng = np.random.default_rng(hd + ratio + news)
+    n_q, n_kv, page, lens = 8, 2, 64, [2000]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.01 * rng.uniform(0.7, 1.4, cache["ks"].shape)
+    cache["vs"][:] = 0.5 * rng.uniform(0.7, 1.4, cache["vs"].shape)
+    q = rng.standard_normal((news, n_q, hd))
+    if ratio:
+        cache["kc"][..., 5] = 0
+        q = _strong(rng, q, ratio)
+    q = q.astype(np.float16)
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len)
+    want, _ = _attend(cache, q, [0, news], lens, table, n_kv)
+    rel = math.sqrt(np.mean((got - want) ** 2) / np.mean(want ** 2))
+    print(f"[precision] {kind} {hd} {ratio}: relative error {rel:.2e}", flush=True)
+    assert rel <= 2.82e-4 * (1 if kind != "wide" else math.sqrt(2)) + 1e-5
