@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     if (t == 0) s_bad = 0;
     __syncthreads();
 
-    // ---- prefix sums, kPlanPer consecutive requests a thread
+    // ---- prefix sums, `per` consecutive requests a thread
     const int per = (n + kPlanThreads - 1) / kPlanThreads, r0 = min(n, t * per), r1 = min(n, r0 + per);
     int64_t rows = 0, take = 0, give = 0;
     int bad = 0;
@@ -128,8 +128,9 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     const int hm = bad ? 0 : (int)(head % a.n_pages), tm = bad ? 0 : (int)(tail % a.n_pages);
     auto ring_at = [&](int base, int i) { return base < a.n_pages - i ? base + i : base - (a.n_pages - i); };
     auto blocks_of = [&](int len) { return (int)(((int64_t)len + page - 1) >> a.pshift); };
-    const int end = min(a.max_rows, ((int)blockIdx.x + 1) * kPlanRows);
-    for (int i = (int)blockIdx.x * kPlanRows + t; i < end; i += kPlanThreads) {
+    const int first = (int)blockIdx.x * kPlanRows, n_own = min(a.max_rows - first, kPlanRows);   // (up to 2^31 - 1 rows)
+    for (int o = t; o < n_own; o += kPlanThreads) {
+        const int i = first + o;
         int p = -1;
         int64_t slot = -1;
         if (i < live) {
@@ -631,7 +632,7 @@ int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, 
     // 18.4 for 16.6 with pages of 128), 1,000 decode rows 29.2 us (a row a workgroup 34.9)
     const int per = page < 64 ? 64 / page : 1;   // heads a workgroup takes
     a.window = rows <= 256 ? 1 : rows <= 2048 ? 4 / per : 32;
-    const unsigned windows = (unsigned)((rows + a.window - 1) / a.window);
+    const unsigned windows = ((unsigned)rows + a.window - 1) / a.window;
     if ((n_kv + per - 1) / per > 65535) return fail(BX_EUNSUPPORTED, "kv_append_q8: too many heads");
     const dim3 grid(windows, (unsigned)((n_kv + per - 1) / per), 2);
     hipStream_t st = as_stream(stream);

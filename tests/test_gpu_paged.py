@@ -189,6 +189,27 @@ def test_plan_pages_outside_the_pool():
     release()
 
 
+def test_plan_most_rows():
+    """A step of 2^31 - 1 rows at most: those behind the last one are all marked."""
+    t = torch()
+    page, rows = 64, 2 ** 31 - 1
+    d = Plan(2, page, 8, 4, 1, np.arange(8, dtype=np.int32), np.array([0, 8], np.int64), np.full((2, 4), -1, np.int32),
+             np.zeros(2, np.int32))
+    d.max_rows = rows
+    d.slots = t.full((rows,), 77, dtype=t.int64, device="cuda")
+    d.pos = t.full((rows,), 77, dtype=t.int32, device="cuda")
+    d.step(dev(np.array([3, 70], np.int32)))
+    assert host(d.status)[0] == 0
+    np.testing.assert_array_equal(host(d.pos[:73]), list(range(3)) + list(range(70)))
+    np.testing.assert_array_equal(host(d.slots[:73]), list(range(3)) + list(range(64, 64 + 70)))
+    for x in (d.pos, d.slots):
+        for a in range(73, rows, 1 << 28):
+            assert bool((x[a:a + (1 << 28)] == -1).all()), a
+    del d, x
+    release()
+    t.cuda.empty_cache()
+
+
 # ----------------------------------------------------------- append and read
 
 @pytest.mark.parametrize("n_kv,hd,page", [(1, 64, 16), (2, 128, 64), (3, 256, 32), (8, 128, 128), (2, 64, 128), (5, 128, 16)])
