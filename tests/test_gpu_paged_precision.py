@@ -195,3 +195,54 @@ def test_relative_error(kind, news, max_new, max_len, ratio, hd):
     rel = math.sqrt(np.mean((got - want) ** 2) / np.mean(want ** 2))
     print(f"[precision] {kind} {hd} {ratio}: relative error {rel:.2e}", flush=True)
     assert rel <= 2.82e-4 * (1 if kind != "wide" else math.sqrt(2)) + 1e-5
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd,page,lens,news", [
+    (8, 2, 256, 16, [900, 1, 330], [70, 1, 40]), (4, 1, 256, 128, [900, 1, 330], [70, 1, 40]),
+    (8, 2, 64, 32, [1100, 700, 64], [150, 90, 2]), (8, 1, 128, 64, [1100, 40], [33, 40])])
+@pytest.mark.parametrize("window", [0, 250])
+def test_chunks_of_many_tiles(n_q, n_kv, hd, page, lens, news, window):
+    """Tiles of 128 columns over contexts of many tiles of keys, in several parts that are joined."""
+    rng = np.random.default_rng(sum(lens) + window)
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.01 * rng.uniform(0.7, 1.4, cache["ks"].shape)
+    cache["vs"][:] = 0.02 * 2.0 ** -rng.choice([0, 0, 1, 5], cache["vs"].shape)
+    starts = np.concatenate([[0], np.cumsum(news)])
+    q = rng.standard_normal((int(starts[-1]), n_q, hd)).astype(np.float16)
+    got = _run(cache, q, starts, lens, table, n_q, max(news) + 65, 1 << 21, window)
+    again = _run(cache, q, starts, lens, table, n_q, max(news) + 65, 1 << 21, window)
+    want, bound = _attend(cache, q, starts, lens, table, n_kv, window, pair=False)
+    _within(got, want, bound, "chunks")
+    np.testing.assert_array_equal(got, again)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 1111])
+@pytest.mark.parametrize("kind,news,length,max_new,max_len", [
+    ("one", 1, 9000, 1, 9000), ("one", 3, 2500, 4, 9000), ("narrow", 32, 3000, 32, 3000), ("wide", 70, 3000, 135, 1 << 21)])
+def test_every_key_counts_once(kind, news, length, max_new, max_len, window, hd):
+    """Values with one head dim each, so that an output is the sum of a few weights: one key lost
+    or counted twice, at a tile's, a part's or the window's edge, is far outside the bound."""
+    rng = np.random.default_rng(hd + length + window)
+    n_q, n_kv, page, lens = 4, 1, 64, [length]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.001
+    cache["vs"][:] = 0.01
+    cache["vc"][:] = 0
+    key = np.arange(length)
+    cache["vc"][table[0, key // page], 0, (7 * key + key // hd) % hd, key % page] = 100
+    q = rng.standard_normal((news, n_q, hd)).astype(np.float16)
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len, window)
+    want, bound = _attend(cache, q, [0, news], lens, table, n_kv, window, pair=kind != "wide")
+    _within(got, want, bound, kind)
+    # the oracle without one key is found out, whichever it is, by every row that sees it
+    at = np.arange(length - news, length)
+    for lost in (length - news, length - 64, length - 65, length - 700, *rng.integers(length - (window or length) + news, length - news, 3)):
+        less = {k: v.copy() for k, v in cache.items()}
+        less["vc"][table[0, lost // page], 0, :, lost % page] = 0
+        off, _ = _attend(less, q, [0, news], lens, table, n_kv, window, pair=kind != "wide")
+        found = (np.abs(off - want) > 2 * bound).any(axis=(1, 2))
+        sees = (at >= lost) & ((at < lost + window) | (window == 0))
+        assert sees.any() and found[sees].all(), lost
