@@ -268,6 +268,44 @@ def test_append_runs(n_kv, hd, page):
     release()
 
 
+@pytest.mark.parametrize("n_kv,hd,page", [(3, 64, 16), (3, 128, 32), (3, 64, 64), (1, 128, 128), (2, 256, 64), (5, 64, 32)])
+def test_append_runs_of_long_prompts(n_kv, hd, page):
+    """More than 2,048 rows in a call, runs of every length at every place of a page: several
+    runs, short and long, begin in one workgroup's share of the rows, and long ones leave it."""
+    rng = np.random.default_rng(hd + page + n_kv)
+    n_pages = 6000 // page + 120
+    want = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    c = Cache(want)
+    filled = np.zeros(n_pages, int)
+    for step in range(3):
+        slots = []
+        for pg in rng.permutation(n_pages):
+            n = min(page - filled[pg], int(rng.choice([1, 2, 7, 15, 16, 17, page - 1, page], p=[.15, .1, .1, .1, .1, .1, .1, .25])))
+            if n == 0:
+                filled[pg] = 0   # the page starts over
+                n = int(rng.integers(1, page + 1))
+            slots += list(pg * page + filled[pg] + np.arange(n))
+            filled[pg] += n
+            if rng.random() < 0.2:
+                slots += [-1] * int(rng.integers(1, 4))
+        slots = np.array(slots, np.int64)
+        rows = slots.size
+        assert rows > 2048
+        size = rng.choice([0.0, 1e-3, 1.0, 30.0], (rows, 1, 1), p=[0.1, 0.2, 0.5, 0.2])
+        k, v = ((rng.standard_normal((rows, n_kv, hd)) * size).astype(np.float16) for _ in range(2))
+        print(f"[append] n_kv={n_kv} hd={hd} page={page} step={step} rows={rows}", flush=True)
+        c.append(f16_dev(k), f16_dev(v), dev(slots))
+        pu.append(want, k, v, slots)
+        got = c.host()
+        np.testing.assert_array_equal(got["ks"], want["ks"])
+        np.testing.assert_array_equal(got["vs"], want["vs"])
+        for pg in range(n_pages):
+            n = filled[pg]
+            np.testing.assert_array_equal(got["kc"][pg][:, :n], want["kc"][pg][:, :n])
+            np.testing.assert_array_equal(got["vc"][pg][:, :, :n], want["vc"][pg][:, :, :n])
+    release()
+
+
 def test_append_rounds_ties_to_even():
     """Codes that fall exactly between two integers, new and requantized."""
     page, hd = 16, 64
