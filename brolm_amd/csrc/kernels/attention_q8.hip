@@ -29,7 +29,8 @@
 // leaves a record (O, m, l), the last one to arrive adds them in split order.
 //
 // Single tokens are bound by their bytes: 48 requests of 8,000 to 16,000 keys, 8 KV heads of
-// 128, 5.6 TB/s of codes; one of 700 keys by latency (9.7 us: lengths, table, rows, the merge).
+// 128, 212 us, 5.6 TB/s of codes (8 heads of 64: 107 us, 5.4; 4 of 256: 260 us, 4.4, one
+// wavefront a SIMD); one of 700 keys by latency (9.8 us: lengths, table, rows, the merge).
 #include <algorithm>
 
 #include "gemm_job.h"
@@ -603,13 +604,14 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
 // two tiles ahead, converts them once for the 128 columns and stores them double-buffered
 // (one barrier a tile; 16-byte chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with
 // q as it is.
-// Two prompts of 2,047 rows, 32 / 8 heads of 128: 102 to 110 us, 600 to 655 TFLOP/s; 1,500 rows
-// at 12,000 keys 800.  What bounds it: two wavefronts a SIMD (240 registers, 64 KB of LDS a
-// workgroup), whose VALU work (exponents, exponentials, sums and the conversion of codes,
-// about 290 instructions a tile beside 64 matrix instructions) fills 60 % of the time, the
-// matrix cores 27 %, and 27 % of whose cycles wait, mostly at the tile's barrier.  Eight
-// wavefronts that share a tile convert half as much for 5 % and leave a batch half as many
-// workgroups; holding the next tile's conversion over the softmax spills (194 us).
+// Prompts of 2,047 and 2,010 rows, 32 / 8 heads of 128: 101 us, 667 TFLOP/s (heads of 64: 72 us;
+// 16 / 4 heads of 256: 166); 1,500 rows at 12,000 keys 800.  What bounds it: two wavefronts a
+// SIMD (245 registers, 64 KB of LDS a workgroup), whose VALU work (exponents, exponentials,
+// sums and the conversion of codes, about 360 instructions for every 64 matrix instructions)
+// fills 59 % of the time, the matrix cores a quarter, and 28 % of whose cycles wait, for
+// counters or at the tile's barrier.  Eight wavefronts that share a tile convert half as much
+// for 5 % and leave a batch half as many workgroups; holding the next tile's conversion over
+// the softmax spills (194 us).  Heads of 256 spill as it is (30 registers), at one wavefront a SIMD.
 template <int HD>
 struct QrShape {
     static constexpr int CH = HD / 8;             // 16-byte chunks of a K row
@@ -982,7 +984,8 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         // against 128: 48 requests of 8,000 to 16,000 keys, 8 rows each 313 and 471 us, 12 411
         // and 578; 16 of 750 to 1,500, 8 rows 17.0 and 29.4, 16 rows 25.3 and 35.8, 32 rows
         // 42.2 and 41.7; one of 8,000, 64 rows 33.6 and 41.4; one prompt of 300, 16 / 8
-        // heads 10.8 and 16.8, of 1,000 27.2 and 26.8.
+        // heads 10.8 and 16.8, of 1,000 27.2 and 26.8.  (Above kQaNarrowReq requests a few rows each
+        // go to tiles of 128: 256 requests of 750 to 1,500 keys, 8 rows each, 183 us, 257 of them 244.)
         const int64_t likely = n_req - longer + ((more + longer) * G + 15) / 16;
         if ((int64_t)max_new * G <= kQaNarrowCols || likely * n_kv * max_len <= kQaNarrowWork / hd) {
             small(n_req + (int64_t)rows * G / 16, likely);

@@ -200,9 +200,10 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
 // step's rows) is one wavefront's; for a longer one the four wavefronts of a workgroup are
 // the units of the page (and of 4 / (units) heads where a page has fewer) and share its
 // amax through LDS.
-// 16 rows of 8 heads of 128: 4.3 us, slots, scale and rows, stores in series.  Three prompts of
-// 7,389 rows: 15.6 us for 46 MB, 2.9 TB/s: the slots are read before the rows can be, and the
-// rounding is a third of the time (19.7 us with the exact form for every value).
+// 16 rows of 8 heads of 128: 4.4 us, slots, scale and rows, stores in series.  Three prompts of
+// 7,389 rows: 15.6 us for 46 MB, 2.9 TB/s: a workgroup's runs come one after the other, slots,
+// rows, the maximum's barrier, codes, and the rounding is a third of the time (19.7 us with the
+// exact form for every value).  Heads of 256 in pages of 128 spill 13 registers.
 
 typedef u4v __attribute__((aligned(2))) any16;
 typedef u2v __attribute__((aligned(2))) any8;
@@ -478,8 +479,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(Append
 // it takes the pieces of 16 tokens of a page that begin among its rows (a row that
 // is not the next token of the row before it, or the first of a piece): a lane holds
 // 4 head dims of hd / 16 tokens.
-// 203 rows of 8 heads of 128: 4.2 us, slots, then codes and scales.  30,011 rows of 8 heads of
-// 64, 92 MB: 19 us, 4.9 TB/s, a copy's rate.
+// 203 rows of 8 heads of 128: 4.4 us, slots, then codes and scales.  30,011 rows of 8 heads of
+// 64, 92 MB: 26 us from memory, 3.5 TB/s (a copy has 5.2), 20 us where the 256 MB cache still
+// has the codes.
 struct ReadArgs {
     const int64_t* slots;
     int rows, n_kv, pshift;

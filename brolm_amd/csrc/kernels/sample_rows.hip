@@ -18,16 +18,18 @@
 // its level.
 //
 // The exponentials are 2^(n / 64) from a table times a polynomial of degree 5 in the
-// rest (a table-driven reduction, relative error below 2^-50), and of four neighbouring
-// keys one only: keys of one exponent are evenly spaced, so each weighs a constant
-// times the next.
+// rest (a table-driven reduction, relative error below 2^-50, to which the rounding of the
+// argument adds (max - l) / T 2^-52), and of four neighbouring keys one only: keys of one
+// exponent are evenly spaced, so each weighs a constant times the next.
 //
 // 16 rows of 151,936 ids: 31 us, 200 rows: 39.  What bounds it: one CU a row, whose LDS makes
 // 64 additions in about 16 cycles (15 us a row), the levels' exponentials (6 us), and the two
 // looks at the row.
 //
 // A 16-bit count wraps for more than 65,535 equal logits; the counts then add up
-// to less than the vocabulary, and the row is done again in pieces that cannot.
+// to less than the vocabulary, and the row is done again in pieces that cannot, and read once
+// more for each cut: 16 rows of 151,936 ids, 100,000 of them at -infinity, 256 us.  (45,000 of
+// them 58 us: their additions meet in one place of the histogram.)
 #include <cmath>
 
 #include "common.h"

@@ -300,7 +300,8 @@ int bx_sample_f16(const uint16_t* logits, int vocab, float temperature, int top_
  * first id stays in any case.  Drawn is the first id where the running kept mass
  * exceeds u (in [0, 1)) times the kept mass; masses in FP64 from the exact logits /
  * temperature.  A temperature that is not positive takes the first id.  NaN
- * logits count as -infinity; out (rows) device int32.  vocab <= 4,194,304. */
+ * logits count as -infinity; out (rows) device int32.  vocab <= 4,194,304.  A row with
+ * more than 65,535 equal logits (a masked vocabulary) takes several times as long. */
 int bx_sample_rows_f16(const uint16_t* logits, int64_t stride, int rows, int vocab, const float* temperature,
                        const int32_t* top_k, const float* top_p, const float* min_p, const double* u, int32_t* out,
                        void* stream);
@@ -385,8 +386,13 @@ int bx_kv_read_q8_f16(const int64_t* slots, int rows, int n_kv, int hd, int page
  * -> out (rows, n_q*hd), out_stride apart.  Query head h reads KV head h / (n_q /
  * n_kv), n_q / n_kv <= 16.  Rows from starts[n_req] on are left as they are; a row
  * that sees no key (more rows than keys; table entries that name no page hide
- * their keys) gives zeros.  max_new >= every request's rows (a request
- * with more may be left as it is) and max_len (about the longest request) shape the launch.
+ * their keys) gives zeros.  Scores, softmax and sums are FP32.  Single tokens and
+ * short chunks take q to 2^-23 of its head's largest element and the weights times
+ * the V scale, which enter the product with V as FP16, to 2^-22; long chunks take q as
+ * it is and those to 2^-11.  What contributes less than 2^-21 of a row's largest part
+ * has fewer bits.
+ * max_new >= every request's rows (a request with more may be left as it is) and
+ * max_len (about the longest request) shape the launch.
  * ws: bx_attention_paged_q8_workspace_bytes(...) bytes with the same arguments (the
  * largest of these over a program's shapes serves them all; a smaller shape may want more
  * than a larger one), 16-byte aligned, its first 512 KB zeroed once before the first use;
