@@ -246,3 +246,26 @@ def test_every_key_counts_once(kind, news, length, max_new, max_len, window, hd)
         found = (np.abs(off - want) > 2 * bound).any(axis=(1, 2))
         sees = (at >= lost) & ((at < lost + window) | (window == 0))
         assert sees.any() and found[sees].all(), lost
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("kind,news,max_new,max_len", KINDS)
+def test_rows_beside_a_page_without_values(kind, news, max_new, max_len, bad, hd):
+    """The last page's V scale is NaN or infinite for one KV head: the rows before it in the same
+    tile, and the other head, have their values as exactly as ever."""
+    rng = np.random.default_rng(hd + news)
+    n_q, n_kv, page, lens = 4, 2, 16, [50]
+    table, n_pages = _tables(rng, lens, page)
+    cache = pu.empty_cache(n_pages, n_kv, page, hd, rng)
+    cache["ks"][:] = 0.02
+    cache["vs"][:] = 0.02 * 2.0 ** rng.integers(-20, 8, cache["vs"].shape)
+    plain = {k: v.copy() for k, v in cache.items()}
+    cache["vs"][table[0, 3], 1] = bad
+    q = _grid(rng, news, n_q, hd)
+    got = _run(cache, q, [0, news], lens, table, n_q, max_new, max_len)
+    want, bound = _attend(plain, q, [0, news], lens, table, n_kv, pair=kind != "wide")
+    sees = np.zeros((news, n_q), bool)
+    sees[np.arange(50 - news, 50) >= 48, 2:] = True
+    assert sees.any() and not np.isfinite(got[sees]).any()
+    _within(got[~sees], want[~sees], bound[~sees], kind)
