@@ -145,6 +145,13 @@ HIP_SYMBOLS = {
     "bx_attention_paged_q8_f16": (C.c_int, [vp, i64, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int,
                                             C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64, vp,
                                             C.c_size_t, vp]),
+    "bx_prefix_plan": (C.c_int, [vp, vp, vp, vp, C.c_int, vp, vp, vp, vp, C.c_int, vp, vp, vp]),
+    "bx_qkv_append_q8_f16": (C.c_int, [vp, i64, vp, i64, vp, i64, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_float,
+                                       vp, vp, vp, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp, vp, vp, i64, vp]),
+    "bx_attention_prefix_q8_workspace_bytes": (C.c_size_t, [C.c_int] * 9),
+    "bx_attention_prefix_q8_f16": (C.c_int, [vp, i64, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp,
+                                             C.c_int, C.c_int, vp, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, C.c_int,
+                                             C.c_int, C.c_int, C.c_int, vp, i64, vp, C.c_size_t, vp]),
     "bx_linear_group_f16": (C.c_int, [C.c_int, C.c_int, C.POINTER(vp), C.POINTER(vp), C.POINTER(C.c_int), vp, C.c_int,
                                       C.c_int, vp, C.c_size_t, vp]),
     "bx_linear_residual_f16": (C.c_int, [C.c_int, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]),

@@ -79,6 +79,18 @@ struct QaArgs {
     uint32_t tag;
 };
 
+// A step whose requests share prefixes (bx_attention_prefix_q8_f16).  What a row's own keys
+// gave, and each part of the shared ones, is left as (O, m, l) where the row shares any:
+// entry (n rows + row) n_q + head of `part` and `part_ml`, n 0 for the own keys, 1 + s for part
+// s of the shared ones, of which there are part_n[row n_q + head] (the heads of a row may lie in
+// two tiles).
+struct QsArgs : QaArgs {
+    const int32_t *pos, *shared, *order, *groups, *group_starts;
+    int max_groups;
+    float *part, *part_ml;
+    int32_t* part_n;
+};
+
 // The first key that the row at position p sees (p below 0 where there are more rows than
 // keys; the window may be anything up to 2^31 - 1).
 __device__ __forceinline__ int first_key(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
@@ -311,9 +323,10 @@ struct QaTile {
 };
 
 // NT: rows by streaming loads (below, at the launch).
-template <int HD, bool NT>
-__device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigned char* smem) {
+template <int HD, bool NT, class A>
+__device__ __forceinline__ void qa_tile(const A& a, unsigned block, unsigned char* smem) {
     constexpr int NC = HD / 64, NJ = HD / 16;
+    constexpr bool PART = std::is_same_v<A, QsArgs>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
@@ -518,6 +531,16 @@ __device__ __forceinline__ void qa_tile(const QaArgs& a, unsigned block, unsigne
     }
     auto store = [&](float sum) {
         if (!real) return;
+        if constexpr (PART) {
+            if (a.shared[row0 + tok] > 0) {
+                const int64_t at = (int64_t)(row0 + tok) * (a.n_kv * G) + head;
+#pragma unroll
+                for (int jj = 0; jj < NJ / 4; ++jj)
+                    *reinterpret_cast<qa_f4*>(a.part + at * HD + 16 * (wave + 4 * jj) + 4 * lg) = acc[jj];
+                if (wave == 0 && lg == 0) *reinterpret_cast<f2v*>(a.part_ml + 2 * at) = f2v{M, sum};
+                return;
+            }
+        }
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
         uint16_t* const orow = a.out + (int64_t)(row0 + tok) * a.out_stride + (int64_t)head * HD + 4 * lg;
 #pragma unroll
@@ -629,10 +652,22 @@ struct QrShape {
     static __device__ __forceinline__ int vswz(int d) { return (d >> 1) & 7; }
 };
 
-template <int HD>
-__device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, unsigned blocks, unsigned char* smem) {
+// Over all lanes of a row of 16, in each of them.
+template <class F>
+__device__ __forceinline__ int row16_of(int v, F&& op) {
+    v = op(v, (int)dpp_of<0xB1>((uint32_t)v));
+    v = op(v, (int)dpp_of<0x4E>((uint32_t)v));
+    v = op(v, (int)dpp_of<0x141>((uint32_t)v));
+    return op(v, (int)dpp_of<0x140>((uint32_t)v));
+}
+
+// SHARED: columns are the rows that share the keys of one request (a group of the plan), 128
+// of them a tile, each with its own last key; what each part gave is left for the join.
+template <int HD, bool SHARED, class A>
+__device__ __forceinline__ void qa_rows_tile(const A& a, unsigned block, unsigned blocks, unsigned char* smem) {
     using S = QrShape<HD>;
     constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI, KB = HD > 128 ? 1 : 2;
+    constexpr bool PART = std::is_same_v<A, QsArgs>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
@@ -641,51 +676,99 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
     const unsigned b = blocks - 1 - block, rest = b / (unsigned)a.n_kv;
     const int g = (int)(b % (unsigned)a.n_kv), s = (int)(rest % (unsigned)a.S);
     const int64_t tile = rest / (unsigned)a.S;
-    int r = 0;
+    const int32_t* const first = [&] {
+        if constexpr (SHARED) return a.group_starts;
+        else return a.starts;
+    }();
+    int r = 0;   // the request; the group
     {
-        int hi = a.n_req;
+        int hi;
+        if constexpr (SHARED) hi = a.max_groups;
+        else hi = a.n_req;
         while (hi - r > 1) {
             const int mid = (r + hi) >> 1;
-            if ((int64_t)a.starts[mid] * G / 128 + mid <= tile) r = mid;
+            if ((int64_t)first[mid] * G / 128 + mid <= tile) r = mid;
             else hi = mid;
         }
     }
-    const int row0 = a.starts[r], n_new = a.starts[r + 1] - row0;
+    const int row0 = first[r], n_new = first[r + 1] - row0;   // SHARED: places in `order`
     const int ti = (int)(tile - ((int64_t)row0 * G / 128 + r));
     if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || ti < 0) return;
     const int64_t ncol = (int64_t)n_new * G, c0 = 128 * (int64_t)ti;
-    if (c0 >= ncol || ncol <= 16) return;   // up to 16 columns are qa_kernel's
+    if (c0 >= ncol || (!SHARED && ncol <= 16)) return;   // up to 16 columns are qa_kernel's
+    if constexpr (SHARED) {
+        r = a.groups[r];
+        if (r < 0 || r >= a.n_req) return;
+    }
     const int len = (int)min((int64_t)max(0, a.lens[r]), (int64_t)a.max_blocks << a.pshift);
     const int p0 = len - n_new;
     auto low = [&](int p) { return first_key(p, a.window); };
-    const int t_first = (int)(c0 / G), t_last = (int)((min(c0 + 128, ncol) - 1) / G);
-    const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
-    const int n64 = max(0, (kend + 63) / 64 - k64);
-    const int ku = max(4, (n64 + a.S - 1) / a.S), T = max(1, (n64 + ku - 1) / ku);
-    if (s >= T) return;
-    const int tb = s * ku, te = min(n64, tb + ku);
 
-    // ---- this wavefront's columns: fragment f, lane l: column 16 f + l % 16 of its 32
+    // ---- this wavefront's columns: fragment f, lane l: column 16 f + l % 16 of its 32;
+    // they see keys plow .. plast
     const int64_t w0 = c0 + 32 * wave;
     const bool works = w0 < ncol;
     bool real[2];
-    int tok[2], head[2], plast[2], plow[2];
+    int row[2], head[2], plast[2], plow[2];
     qa_h8 qf[2][NS];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
         const int64_t c = w0 + 16 * f + lc;
         real[f] = c < ncol;
         const int64_t cc = real[f] ? c : c0;
-        tok[f] = (int)(cc / G);
+        const int tok = (int)(cc / G);
         head[f] = g * G + (int)(cc % G);
-        plast[f] = real[f] ? p0 + tok[f] : -1;
-        plow[f] = low(p0 + tok[f]);
-        const uint16_t* const q = a.q + (int64_t)(row0 + tok[f]) * a.q_stride + (int64_t)head[f] * HD + 8 * lg;
+        if constexpr (SHARED) {
+            row[f] = a.order[row0 + tok];
+            if (row[f] < 0 || row[f] >= a.rows) {
+                real[f] = false;
+                row[f] = 0;
+            }
+            plast[f] = real[f] ? min(a.shared[row[f]], len) - 1 : -1;
+            plow[f] = low(a.pos[row[f]]);
+        } else {
+            row[f] = row0 + tok;
+            plast[f] = real[f] ? p0 + tok : -1;
+            plow[f] = low(p0 + tok);
+        }
+        const uint16_t* const q = a.q + (int64_t)row[f] * a.q_stride + (int64_t)head[f] * HD + 8 * lg;
 #pragma unroll
         for (int d = 0; d < NS; ++d)
             qf[f][d] = __builtin_bit_cast(qa_h8, (u4v)*reinterpret_cast<const qa_any16*>(q + 32 * d));
     }
-    const int w_first = p0 + (int)(min(w0, ncol - 1) / G), w_last = p0 + (int)((min(w0 + 32, ncol) - 1) / G);
+    // the least and the greatest of the wavefront's first and last keys, and of the tile's
+    int low_min, low_max, last_min, last_max, kend, k64;
+    if constexpr (SHARED) {
+        auto mn = [](int x, int y) { return min(x, y); };
+        auto mx = [](int x, int y) { return max(x, y); };
+        constexpr int kMost = 0x7fffffff;
+        low_min = __builtin_amdgcn_readfirstlane(row16_of(min(real[0] ? plow[0] : kMost, real[1] ? plow[1] : kMost), mn));
+        low_max = __builtin_amdgcn_readfirstlane(row16_of(max(real[0] ? plow[0] : 0, real[1] ? plow[1] : 0), mx));
+        last_min = __builtin_amdgcn_readfirstlane(row16_of(min(real[0] ? plast[0] : kMost, real[1] ? plast[1] : kMost), mn));
+        last_max = __builtin_amdgcn_readfirstlane(row16_of(max(plast[0], plast[1]), mx));
+        int* const ends = reinterpret_cast<int*>(smem);
+        if (lane == 0) {
+            ends[wave] = low_min;
+            ends[4 + wave] = last_max;
+        }
+        __syncthreads();
+        kend = max(max(ends[4], ends[5]), max(ends[6], ends[7])) + 1;
+        k64 = min(min(min(ends[0], ends[1]), min(ends[2], ends[3])), kend) / 64;
+        __syncthreads();   // the tiles go there
+    } else {
+        const int t_first = (int)(c0 / G), t_last = (int)((min(c0 + 128, ncol) - 1) / G);
+        const int w_first = p0 + (int)(min(w0, ncol - 1) / G), w_last = p0 + (int)((min(w0 + 32, ncol) - 1) / G);
+        kend = max(0, p0 + t_last + 1);
+        k64 = low(p0 + t_first) / 64;
+        low_min = low(w_first);
+        low_max = low(w_last);
+        last_min = w_first;
+        last_max = w_last;
+    }
+    const int n64 = max(0, (kend + 63) / 64 - k64);
+    const int ku = max(4, (n64 + a.S - 1) / a.S), T = max(1, (n64 + ku - 1) / ku);
+    if (s >= T) return;
+    const int tb = s * ku, te = min(n64, tb + ku);
 
     // ---- tiles through registers: piece i of a thread is 16 codes of key 16 grp + .. (K)
     // and of head dim .. (V) of the 16 keys grp = thread / HD + i (256 / HD)
@@ -777,7 +860,7 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
         ok = ok2;
         scales();   // of the next tile
         look(i + 2);
-        if (works && key <= w_last && key + 63 >= low(w_first)) {
+        if (works && key <= last_max && key + 63 >= low_min) {
             // fragments from LDS a step ahead of the products that take them (heads of 256
             // have no registers for K's)
             float y[2][4][4];
@@ -804,9 +887,9 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y[f][t][e] = acc[f][e];
             }
-            const bool whole = key + 63 <= w_first && key >= low(w_last) && __all(ok);
+            const bool whole = key + 63 <= last_min && key >= low_max && __all(ok);
             const int kk = key + 16 * lg;
-            sc.next(sv, ok && kk <= w_last && kk + 15 >= low(w_first));
+            sc.next(sv, ok && kk <= last_max && kk + 15 >= low_min);
             qa_h8 pb[2][2];
             qa_softmax<2, false>(
                 y, sk, cfs, !whole,
@@ -844,10 +927,35 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
     }
 #pragma unroll
     for (int f = 0; f < 2; ++f) l[f] = quad_sum(l[f]);
-    auto store = [&](int f, float sum) {
+    // entry n of a row that shares keys
+    auto leave = [&](int n, int f, float max, float sum) {
+        if constexpr (PART) {
+            const int64_t at = ((int64_t)n * a.rows + row[f]) * (a.n_kv * G) + head[f];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) *reinterpret_cast<qa_f4*>(a.part + at * HD + 16 * j + 4 * lg) = o[f][j];
+            if (lg == 0) *reinterpret_cast<f2v*>(a.part_ml + 2 * at) = f2v{max, sum};
+        }
+    };
+    if constexpr (SHARED) {
+        if (works)
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+                if (real[f]) {
+                    leave(1 + s, f, m[f], l[f]);
+                    if (s == 0 && lg == 0) a.part_n[(int64_t)row[f] * (a.n_kv * G) + head[f]] = T;
+                }
+        return;
+    }
+    auto store = [&](int f, float max, float sum) {
         if (!real[f]) return;
+        if constexpr (PART) {
+            if (a.shared[row[f]] > 0) {
+                leave(0, f, max, sum);
+                return;
+            }
+        }
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        uint16_t* const orow = a.out + (int64_t)(row0 + tok[f]) * a.out_stride + (int64_t)head[f] * HD + 4 * lg;
+        uint16_t* const orow = a.out + (int64_t)row[f] * a.out_stride + (int64_t)head[f] * HD + 4 * lg;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             u2v w;
@@ -858,8 +966,8 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
     };
     if (T == 1) {
         if (works) {
-            store(0, l[0]);
-            store(1, l[1]);
+            store(0, m[0], l[0]);
+            store(1, m[1], l[1]);
         }
         return;
     }
@@ -919,8 +1027,8 @@ __device__ __forceinline__ void qa_rows_tile(const QaArgs& a, unsigned block, un
             for (int j = 0; j < NJ; ++j) o[f][j] += __builtin_bit_cast(qa_f4, ov[f][j]) * w;
         }
     }
-    store(0, L[0]);
-    store(1, L[1]);
+    store(0, M[0], L[0]);
+    store(1, M[1], L[1]);
 }
 
 template <int HD, bool NT>
@@ -934,8 +1042,61 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
 template <int HD>
 __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_both_kernel(QaArgs rows, QaArgs a, unsigned row_blocks) {
     extern __shared__ __align__(16) unsigned char smem[];
-    if (blockIdx.x < row_blocks) qa_rows_tile<HD>(rows, blockIdx.x, row_blocks, smem);
+    if (blockIdx.x < row_blocks) qa_rows_tile<HD, false>(rows, blockIdx.x, row_blocks, smem);
     else qa_tile<HD, false>(a, blockIdx.x - row_blocks, smem);
+}
+
+// A step with shared prefixes in one launch: tiles of the shared keys, which are the longest,
+// then those of the own keys as above.
+template <int HD>
+__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qs_kernel(QsArgs shared, QsArgs rows, QsArgs a,
+                                                                         unsigned shared_blocks, unsigned row_blocks) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    unsigned b = blockIdx.x;
+    if (b < shared_blocks) return qa_rows_tile<HD, true>(shared, b, shared_blocks, smem);
+    b -= shared_blocks;
+    if (b < row_blocks) return qa_rows_tile<HD, false>(rows, b, row_blocks, smem);
+    qa_tile<HD, false>(a, b - row_blocks, smem);
+}
+
+// Joins what the own keys and the parts of the shared ones gave, a wavefront to a row and
+// head, in the order of the parts.
+template <int HD>
+__global__ __launch_bounds__(kQaThreads) void qs_join_kernel(QsArgs a) {
+    constexpr int LR = HD / 4, R = 64 / LR, B = 4;   // lanes a part, parts at once, loads on their way
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_q = a.n_kv * a.G;
+    const int64_t item = (int64_t)blockIdx.x * 4 + wave, row = item / n_q;
+    if (row >= a.rows || a.shared[row] <= 0) return;
+    const int head = (int)(item - row * n_q);
+    const int n = 1 + min(max(a.part_n[item], 0), a.S);
+    const int64_t step = (int64_t)a.rows * n_q;   // entries from one part to the next
+    f2v ml{-INFINITY, 0.f};
+    if (lane < n) ml = *reinterpret_cast<const f2v*>(a.part_ml + 2 * (lane * step + item));
+    const float M = wave_max(ml.x), w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+    const float sum = wave_sum(w * ml.y);
+    qa_f4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int t0 = 0; t0 < n; t0 += B * R) {
+        qa_f4 o[B];
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            o[u] = *reinterpret_cast<const qa_f4*>(a.part + (min(t0 + u * R + lane / LR, n - 1) * step + item) * HD + 4 * (lane % LR));
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+            const int t = t0 + u * R + lane / LR;
+            const float wt = __shfl(w, min(t, n - 1));
+            if (t < n) acc += o[u] * wt;
+        }
+    }
+#pragma unroll
+    for (int x = LR; x < 64; x *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], x);
+    if (lane >= LR) return;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    u2v y;
+    y.x = (uint32_t)f2h(acc[0] * inv) | ((uint32_t)f2h(acc[1] * inv) << 16);
+    y.y = (uint32_t)f2h(acc[2] * inv) | ((uint32_t)f2h(acc[3] * inv) << 16);
+    *reinterpret_cast<qa_any8*>(a.out + row * a.out_stride + (int64_t)head * HD + 4 * lane) = y;
 }
 
 // How a call is laid out.  Requests of up to 16 columns: a tile each in qa_kernel, their
@@ -1026,6 +1187,39 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     return p;
 }
 
+// A step with shared prefixes: the own keys as above, the shared ones in `tiles` of 128 columns
+// at most, the keys of each over S workgroups.
+constexpr int kQsMaxSplits = 63;   // and the own keys: a lane each in the join
+
+struct QsPlan {
+    QaPlan own;
+    int groups, S;
+    int64_t tiles;
+    size_t part_bytes, ml_bytes, n_bytes;
+    size_t bytes() const { return own.bytes() + part_bytes + ml_bytes + n_bytes; }
+};
+
+QsPlan qs_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len, int max_groups, int max_shared) {
+    QsPlan p{};
+    p.own = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
+    const int64_t G = n_q / n_kv, cus = num_cus(), slots = hd > 128 ? cus : 2 * cus;
+    p.groups = std::min({max_groups, n_req, rows});
+    p.tiles = (int64_t)rows * G / 128 + p.groups;
+    const int64_t likely = (((int64_t)rows * G + 127) / 128 + p.groups - 1) * n_kv, each = (int64_t)rows * n_q * hd * 4;
+    const int64_t cap = std::max<int64_t>(1, std::min<int64_t>({((int64_t)max_shared + 255) / 256, kQsMaxSplits, kQaRecBytes / each}));
+    p.S = (int)std::max<int64_t>(1, std::min(slots / likely, cap));
+    auto up = [](int64_t x) { return ((size_t)x + 255) / 256 * 256; };
+    p.part_bytes = up(each * (1 + p.S));
+    p.ml_bytes = up((int64_t)rows * n_q * 8 * (1 + p.S));
+    p.n_bytes = up((int64_t)rows * n_q * 4);
+    return p;
+}
+
+bool qs_shape_ok(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len, int max_groups, int max_shared) {
+    return rows > 0 && n_req > 0 && n_kv > 0 && n_q > 0 && n_q % n_kv == 0 && hd > 0 && max_new > 0 && max_len > 0 &&
+           max_groups > 0 && max_shared > 0;
+}
+
 }  // namespace
 }  // namespace bx
 
@@ -1099,6 +1293,78 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
             kernel<<<(unsigned)blocks, kQaThreads, lds, st>>>(a);
         }
         return launch_check("attention_paged_q8");
+    };
+    if (hd == 64) return run(std::integral_constant<int, 64>{});
+    if (hd == 128) return run(std::integral_constant<int, 128>{});
+    return run(std::integral_constant<int, 256>{});
+}
+
+size_t bx_attention_prefix_q8_workspace_bytes(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len,
+                                              int max_groups, int max_shared) {
+    if (!qs_shape_ok(rows, n_req, n_q, n_kv, hd, max_new, max_len, max_groups, max_shared)) return 0;
+    return qs_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len, max_groups, max_shared).bytes();
+}
+
+int bx_attention_prefix_q8_f16(const uint16_t* q, int64_t q_stride, int rows, const int32_t* starts, const int32_t* lens,
+                               int n_req, int max_new, int max_len, const int32_t* pos, const int32_t* shared,
+                               const int32_t* order, const int32_t* groups, const int32_t* group_starts, int max_groups,
+                               int max_shared, const int32_t* table, int max_blocks, int page, int n_pages,
+                               const int8_t* Kc, const int8_t* Vc, const float* k_scale, const float* v_scale, int n_q,
+                               int n_kv, int hd, int window, uint16_t* out, int64_t out_stride, void* ws, size_t ws_bytes,
+                               void* stream) {
+    if (!q || !starts || !lens || !pos || !shared || !order || !groups || !group_starts || !table || !out || !ws)
+        return fail(BX_EINVAL, "attention_prefix_q8: null pointer");
+    if (int rc = kv_cache_check("attention_prefix_q8", n_kv, hd, page, n_pages, Kc, Vc, k_scale, v_scale)) return rc;
+    if (!qs_shape_ok(rows, n_req, n_q, n_kv, hd, max_new, max_len, max_groups, max_shared) || max_blocks <= 0 || window < 0)
+        return fail(BX_EINVAL, "attention_prefix_q8: bad shape");
+    if (n_q / n_kv > kQaMaxGroup) return fail(BX_EUNSUPPORTED, "attention_prefix_q8: GQA group larger than 16");
+    if (q_stride < (int64_t)n_q * hd || out_stride < (int64_t)n_q * hd)
+        return fail(BX_EINVAL, "attention_prefix_q8: row stride below n_q * head_dim");
+    if ((int64_t)max_blocks * page > 0x7fffffff - 4095)   // the tiles asked for ahead lie below 2^31 too
+        return fail(BX_EUNSUPPORTED, "attention_prefix_q8: more than 2^31 - 4096 tokens a request");
+    const QsPlan p = qs_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len, max_groups, max_shared);
+    if (ws_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(ws) & 15))
+        return fail(BX_EINVAL, "attention_prefix_q8: workspace too small or not 16-byte aligned");
+    const int64_t blocks = p.own.tiles16 * n_kv * p.own.S, rblocks = p.own.tiles * n_kv * p.own.Sr;
+    const int64_t sblocks = p.tiles * n_kv * p.S, joins = ((int64_t)rows * n_q + 3) / 4;
+    if (blocks + rblocks + sblocks > 0x7fffffff || joins > 0x7fffffff)
+        return fail(BX_EUNSUPPORTED, "attention_prefix_q8: too many rows and heads");
+    QsArgs a{};
+    a.q = q; a.q_stride = q_stride; a.rows = rows; a.starts = starts; a.lens = lens; a.n_req = n_req;
+    a.table = table; a.max_blocks = max_blocks; a.pshift = __builtin_ctz((unsigned)page); a.n_pages = n_pages;
+    a.Kc = Kc; a.Vc = Vc; a.ks = k_scale; a.vs = v_scale;
+    a.n_kv = n_kv; a.G = n_q / n_kv; a.window = window; a.out = out; a.out_stride = out_stride;
+    a.pos = pos; a.shared = shared; a.order = order; a.groups = groups; a.group_starts = group_starts;
+    a.max_groups = p.groups;
+    unsigned char* const w = static_cast<unsigned char*>(ws);
+    unsigned char* const parts = w + p.own.bytes();
+    a.part = reinterpret_cast<float*>(parts);
+    a.part_ml = reinterpret_cast<float*>(parts + p.part_bytes);
+    a.part_n = reinterpret_cast<int32_t*>(parts + p.part_bytes + p.ml_bytes);
+    QsArgs ar = a, as = a;
+    a.narrow = p.own.narrow;
+    a.S = p.own.S;
+    a.cnt = reinterpret_cast<uint64_t*>(w);
+    a.recs = w + QaPlan::kCounters;
+    a.tag = next_launch_tag();
+    ar.S = p.own.Sr;
+    ar.cnt = a.cnt + kQaWords;
+    ar.recs = a.recs + p.own.rec_bytes;
+    ar.tag = next_launch_tag();
+    as.S = p.S;
+    hipStream_t st = as_stream(stream);
+    auto run = [&](auto hdc) -> int {
+        constexpr int HD = decltype(hdc)::value, lds = std::max(HD / 16 * 4096 + 512, 2 * QrShape<HD>::kBuf);
+        if constexpr (lds > 64 * 1024) {
+            static std::atomic<uint64_t> allowed{0};
+            if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qs_kernel<HD>), lds, "attention_prefix_q8: LDS attribute"))
+                return rc;
+        }
+        qs_kernel<HD><<<(unsigned)(sblocks + rblocks + blocks), kQaThreads, lds, st>>>(as, ar, a, (unsigned)sblocks,
+                                                                                      (unsigned)rblocks);
+        if (int rc = launch_check("attention_prefix_q8")) return rc;
+        qs_join_kernel<HD><<<(unsigned)joins, kQaThreads, 0, st>>>(as);
+        return launch_check("attention_prefix_q8: join");
     };
     if (hd == 64) return run(std::integral_constant<int, 64>{});
     if (hd == 128) return run(std::integral_constant<int, 128>{});

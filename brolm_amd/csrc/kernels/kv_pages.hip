@@ -7,6 +7,7 @@
 // bytes along hd for Q K^T, 16 bytes along the tokens for P V) are plain 16-byte
 // loads.  One FP32 scale per page, head and matrix: value = code * scale, codes
 // in [-127, 127].
+#include <algorithm>
 #include <type_traits>
 
 #include "kv_pages.h"
@@ -216,6 +217,12 @@ struct AppendArgs {
     const int64_t* slots;
     int8_t* codes[2];
     float* scale[2];
+    // rows of K as a projection leaves them (ROT below): their head norm and rotation
+    const uint16_t* gain;
+    float eps;
+    const int32_t* pos;
+    const float *cos_t, *sin_t;
+    int tab_rows;
 };
 
 // rint(x / s), ties to even; inv is about 1 / s, s > 0 and finite.
@@ -238,16 +245,52 @@ __device__ __forceinline__ uint32_t put_byte(uint32_t w, int i, int c) {
     return (w & ~(0xffu << (8 * i))) | ((uint32_t)(c & 0xff) << (8 * i));
 }
 
+// Eight elements of a head, HD / 8 consecutive lanes holding it: the head's RMSNorm with the
+// lane's gains (norm), then the rotation of pairs (2 i, 2 i + 1) by (c, s), all in FP32, and
+// one rounding to FP16.
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef f4v __attribute__((aligned(4))) any_f4;
+
+template <int HD>
+__device__ __forceinline__ u4v norm_rope8(u4v x, bool norm, const u4v& gain, float eps, const f4v& c, const f4v& s) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = h2f((uint16_t)(x[i / 2] >> (16 * (i & 1))));
+    if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
+        ss += dpp_f<0xB1>(ss, 0.f);
+        ss += dpp_f<0x4E>(ss, 0.f);
+        ss += dpp_f<0x141>(ss, 0.f);
+        if (HD >= 128) ss += dpp_f<0x140>(ss, 0.f);
+        if (HD >= 256) ss += __shfl_xor(ss, 16);
+        const float inv = 1.0f / sqrtf(ss / (float)HD + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * h2f((uint16_t)(gain[i / 2] >> (16 * (i & 1))));
+    }
+    u4v y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_fmaf(f[2 * i], c[i], -(f[2 * i + 1] * s[i]));
+        const float b = __builtin_fmaf(f[2 * i], s[i], f[2 * i + 1] * c[i]);
+        y[i] = (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16);
+    }
+    return y;
+}
+
 // WHICH 0: K, 1: V; NCH units of 16 tokens a page.  SOLO: the run lies inside one unit, head
-// hs of the workgroup's; else hs is not read.
-template <int HD, int WHICH, int NCH, bool SOLO>
-__device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, int64_t slot, int hs, uint32_t* red) {
+// hs of the workgroup's; else hs is not read.  ROT: rows of K get their head norm and rotation
+// first.
+template <int HD, int WHICH, int NCH, bool SOLO, bool ROT>
+__device__ __forceinline__ void append_run(const AppendArgs& a, unsigned by, int row, int n, int64_t slot, int hs,
+                                           uint32_t* red) {
     constexpr int HPW = NCH < 4 ? 4 / NCH : 1;           // heads a workgroup takes
     constexpr int U = NCH > 4 && !SOLO ? NCH / 4 : 1;    // units a wavefront takes
     constexpr int page = 16 * NCH;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (!SOLO) hs = NCH < 4 ? wave / NCH : 0;
-    const int head = (int)blockIdx.y * HPW + hs;
+    const int head = (int)by * HPW + hs;
     const bool there = head < a.n_kv;
     const int off = (int)(slot & (page - 1));
     auto unit = [&](int u) { return SOLO ? off >> 4 : (NCH < 4 ? wave % NCH : wave) + 4 * u; };
@@ -290,6 +333,21 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
             if (has_new[u]) {
 #pragma unroll
                 for (int j = 0; j < KL; ++j) kx[u][j] = *reinterpret_cast<const any16*>(near(t0 + kt + j * KR) + kd);
+                if constexpr (ROT) {
+                    const u4v g = a.gain ? *reinterpret_cast<const any16*>(a.gain + kd) : u4v{0u, 0u, 0u, 0u};
+                    int ps[KL];
+#pragma unroll
+                    for (int j = 0; j < KL; ++j) ps[j] = a.pos[row - off + min(max(t0 + kt + j * KR, off), off + n - 1)];
+#pragma unroll
+                    for (int j = 0; j < KL; ++j) {
+                        const bool in = ps[j] >= 0 && ps[j] < a.tab_rows;
+                        const int64_t at = (int64_t)(in ? ps[j] : 0) * (HD / 2) + kd / 2;
+                        const f4v c = *reinterpret_cast<const any_f4*>(a.cos_t + at);
+                        const f4v s = *reinterpret_cast<const any_f4*>(a.sin_t + at);
+                        kx[u][j] = norm_rope8<HD>(kx[u][j], a.gain != nullptr, g, a.eps, c, s);
+                        if (!in) kx[u][j] = u4v{0u, 0u, 0u, 0u};
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < KL; ++j)
 #pragma unroll
@@ -423,10 +481,10 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int row, int n, 
 }
 
 // Workgroup (window of rows, heads, K or V): the runs that start in its window.
-template <int HD, int NCH>
-__global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(AppendArgs a) {
-    __shared__ uint32_t red[2][4];
-    const int64_t row0 = (int64_t)blockIdx.x * a.window;
+template <int HD, int NCH, bool ROT>
+__device__ __forceinline__ void append_block(const AppendArgs& a, unsigned bx, unsigned by, unsigned bz,
+                                             uint32_t (*red)[4]) {
+    const int64_t row0 = (int64_t)bx * a.window;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int page = 16 * NCH, HPW = NCH < 4 ? 4 / NCH : 1;
     auto slot_at = [&](int64_t r) { return r >= 0 && r < a.rows ? a.slots[r] : -1; };
@@ -448,8 +506,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(Append
         }
         // wavefront w: head w % HPW of the workgroup's, every (4 / HPW)th run
         if (turn++ % (4 / HPW) != wave / HPW) continue;
-        if (blockIdx.z == 0) append_run<HD, 0, NCH, true>(a, (int)(row0 + i), n, slot, wave % HPW, nullptr);
-        else append_run<HD, 1, NCH, true>(a, (int)(row0 + i), n, slot, wave % HPW, nullptr);
+        if (bz == 0) append_run<HD, 0, NCH, true, ROT>(a, by, (int)(row0 + i), n, slot, wave % HPW, nullptr);
+        else append_run<HD, 1, NCH, true, ROT>(a, by, (int)(row0 + i), n, slot, wave % HPW, nullptr);
     }
     if constexpr (NCH == 1) return;   // a page is one unit
     // longer ones: all four, one after the other (red alternates: one barrier a run)
@@ -468,9 +526,70 @@ __global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(Append
                 n += c;
                 if (c < 64) break;
             }
-        if (blockIdx.z == 0) append_run<HD, 0, NCH, false>(a, row, n, slot, 0, red[k]);
-        else append_run<HD, 1, NCH, false>(a, row, n, slot, 0, red[k]);
+        if (bz == 0) append_run<HD, 0, NCH, false, ROT>(a, by, row, n, slot, 0, red[k]);
+        else append_run<HD, 1, NCH, false, ROT>(a, by, row, n, slot, 0, red[k]);
     }
+}
+
+template <int HD, int NCH>
+__global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(AppendArgs a) {
+    __shared__ uint32_t red[2][4];
+    append_block<HD, NCH, false>(a, blockIdx.x, blockIdx.y, blockIdx.z, red);
+}
+
+// ------------------------------------------------- q, k and v of a step in one pass
+//
+// Blocks below kv_blocks are the append's, with the head norm and the rotation of K in
+// registers between the load and the maximum; the others take the rows of q.  A wavefront
+// holds 512 / HD heads of a row at a time, eight elements a lane, `turns` times with the same
+// angles.
+struct QkvArgs {
+    AppendArgs kv;
+    unsigned windows, head_groups, kv_blocks;
+    const uint16_t* q;
+    uint16_t* out;
+    int64_t q_stride, out_stride;
+    const uint16_t* q_gain;
+    int n_q, turns, parts;   // parts: wavefronts a row
+};
+
+template <int HD>
+__device__ __forceinline__ void q_block(const QkvArgs& a, unsigned block) {
+    constexpr int HW = 512 / HD, MAXT = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t item = (int64_t)block * 4 + wave, row = item / a.parts;
+    if (row >= a.kv.rows) return;
+    const int head0 = (int)(item % a.parts) * HW * a.turns + lane / (HD / 8), d = 8 * (lane % (HD / 8));
+    const int ps = a.kv.pos[row];
+    if (ps < 0 || ps >= a.kv.tab_rows) return;
+    const uint16_t* const x = a.q + row * a.q_stride + d;
+    u4v w[MAXT];
+    // heads behind the last one read it again and are not stored
+#pragma unroll
+    for (int i = 0; i < MAXT; ++i)
+        if (i < a.turns) w[i] = *reinterpret_cast<const any16*>(x + (int64_t)min(head0 + i * HW, a.n_q - 1) * HD);
+    const u4v g = a.q_gain ? *reinterpret_cast<const any16*>(a.q_gain + d) : u4v{0u, 0u, 0u, 0u};
+    const f4v c = *reinterpret_cast<const any_f4*>(a.kv.cos_t + (int64_t)ps * (HD / 2) + d / 2);
+    const f4v s = *reinterpret_cast<const any_f4*>(a.kv.sin_t + (int64_t)ps * (HD / 2) + d / 2);
+#pragma unroll
+    for (int i = 0; i < MAXT; ++i) {
+        if (i >= a.turns) break;
+        const u4v y = norm_rope8<HD>(w[i], a.q_gain != nullptr, g, a.kv.eps, c, s);
+        const int head = head0 + i * HW;
+        if (head < a.n_q) *reinterpret_cast<any16*>(a.out + row * a.out_stride + (int64_t)head * HD + d) = y;
+    }
+}
+
+template <int HD, int NCH>
+__global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void qkv_append_kernel(QkvArgs a) {
+    __shared__ uint32_t red[2][4];
+    const unsigned b = blockIdx.x;
+    if (b >= a.kv_blocks) {
+        q_block<HD>(a, b - a.kv_blocks);
+        return;
+    }
+    const unsigned rest = b / a.windows;
+    append_block<HD, NCH, true>(a.kv, b % a.windows, rest % a.head_groups, rest / a.head_groups, red);
 }
 
 // ------------------------------------------------------------------ the read
@@ -572,6 +691,27 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
 
 }  // namespace
 
+namespace {
+
+int heads_of(int page) { return page < 64 ? 64 / page : 1; }   // heads a workgroup of the append takes
+
+AppendArgs append_args(const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride, int rows, int n_kv,
+                       const int64_t* slots, int page, int n_pages, int8_t* Kc, int8_t* Vc, float* ks, float* vs) {
+    AppendArgs a{};
+    a.x[0] = k; a.x[1] = v; a.stride[0] = k_stride; a.stride[1] = v_stride;
+    a.rows = rows; a.n_kv = n_kv; a.pshift = __builtin_ctz((unsigned)page);
+    a.n_slots = (int64_t)n_pages * page;
+    a.slots = slots; a.codes[0] = Kc; a.codes[1] = Vc; a.scale[0] = ks; a.scale[1] = vs;
+    // a row to a workgroup for few rows, as many as it has wavefronts for their heads where
+    // rows are many (decode rows are a wavefront each), 32 for prompts: three of 7,389 rows
+    // together, 8 heads of 128, pages of 64, 15.6 us (16 rows a workgroup 24.0; 64 the same, but
+    // 18.4 for 16.6 with pages of 128), 1,000 decode rows 29.2 us (a row a workgroup 34.9)
+    a.window = rows <= 256 ? 1 : rows <= 2048 ? 4 / heads_of(page) : 32;
+    return a;
+}
+
+}  // namespace
+
 int kv_cache_check(const char* what, int n_kv, int hd, int page, int n_pages, const int8_t* Kc, const int8_t* Vc,
                 const float* ks, const float* vs) {
     if (!Kc || !Vc || !ks || !vs) return fail(BX_EINVAL, std::string(what) + ": null cache pointer");
@@ -623,17 +763,8 @@ int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, 
     if (int rc = kv_cache_check("kv_append_q8", n_kv, hd, page, n_pages, Kc, Vc, k_scale, v_scale)) return rc;
     const int64_t width = (int64_t)n_kv * hd;
     if (rows <= 0 || k_stride < width || v_stride < width) return fail(BX_EINVAL, "kv_append_q8: bad shape");
-    AppendArgs a{};
-    a.x[0] = k; a.x[1] = v; a.stride[0] = k_stride; a.stride[1] = v_stride;
-    a.rows = rows; a.n_kv = n_kv; a.pshift = __builtin_ctz((unsigned)page);
-    a.n_slots = (int64_t)n_pages * page;
-    a.slots = slots; a.codes[0] = Kc; a.codes[1] = Vc; a.scale[0] = k_scale; a.scale[1] = v_scale;
-    // a row to a workgroup for few rows, as many as it has wavefronts for their heads where
-    // rows are many (decode rows are a wavefront each), 32 for prompts: three of 7,389 rows
-    // together, 8 heads of 128, pages of 64, 15.6 us (16 rows a workgroup 24.0; 64 the same, but
-    // 18.4 for 16.6 with pages of 128), 1,000 decode rows 29.2 us (a row a workgroup 34.9)
-    const int per = page < 64 ? 64 / page : 1;   // heads a workgroup takes
-    a.window = rows <= 256 ? 1 : rows <= 2048 ? 4 / per : 32;
+    const AppendArgs a = append_args(k, k_stride, v, v_stride, rows, n_kv, slots, page, n_pages, Kc, Vc, k_scale, v_scale);
+    const int per = heads_of(page);
     const unsigned windows = ((unsigned)rows + a.window - 1) / a.window;
     if ((n_kv + per - 1) / per > 65535) return fail(BX_EUNSUPPORTED, "kv_append_q8: too many heads");
     const dim3 grid(windows, (unsigned)((n_kv + per - 1) / per), 2);
@@ -649,6 +780,47 @@ int bx_kv_append_q8_f16(const uint16_t* k, int64_t k_stride, const uint16_t* v, 
     else if (hd == 128) run(std::integral_constant<int, 128>{});
     else run(std::integral_constant<int, 256>{});
     return launch_check("kv_append_q8");
+}
+
+int bx_qkv_append_q8_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                         int64_t v_stride, int rows, int n_q, int n_kv, int hd, const uint16_t* q_gain,
+                         const uint16_t* k_gain, float eps, const int32_t* pos, const float* cos_tab,
+                         const float* sin_tab, int tab_rows, const int64_t* slots, int page, int n_pages, int8_t* Kc,
+                         int8_t* Vc, float* k_scale, float* v_scale, uint16_t* q_out, int64_t q_out_stride, void* stream) {
+    if (!q || !k || !v || !pos || !cos_tab || !sin_tab || !slots || !q_out)
+        return fail(BX_EINVAL, "qkv_append_q8: null pointer");
+    if (int rc = kv_cache_check("qkv_append_q8", n_kv, hd, page, n_pages, Kc, Vc, k_scale, v_scale)) return rc;
+    const int64_t width = (int64_t)n_kv * hd, q_width = (int64_t)n_q * hd;
+    if (rows <= 0 || n_q <= 0 || tab_rows <= 0 || k_stride < width || v_stride < width || q_stride < q_width ||
+        q_out_stride < q_width)
+        return fail(BX_EINVAL, "qkv_append_q8: bad shape");
+    if ((q_gain == nullptr) != (k_gain == nullptr)) return fail(BX_EINVAL, "qkv_append_q8: one of two gains");
+    if (!(eps >= 0.f)) return fail(BX_EINVAL, "qkv_append_q8: bad eps");
+    QkvArgs a{};
+    a.kv = append_args(k, k_stride, v, v_stride, rows, n_kv, slots, page, n_pages, Kc, Vc, k_scale, v_scale);
+    a.kv.gain = k_gain; a.kv.eps = eps; a.kv.pos = pos; a.kv.cos_t = cos_tab; a.kv.sin_t = sin_tab; a.kv.tab_rows = tab_rows;
+    const int per = heads_of(page), at_once = 512 / hd;
+    a.windows = ((unsigned)rows + a.kv.window - 1) / a.kv.window;
+    a.head_groups = (unsigned)((n_kv + per - 1) / per);
+    a.q = q; a.q_stride = q_stride; a.out = q_out; a.out_stride = q_out_stride; a.q_gain = q_gain; a.n_q = n_q;
+    const int steps = (n_q + at_once - 1) / at_once;
+    a.turns = rows <= 256 ? 1 : std::min(4, steps);
+    a.parts = (steps + a.turns - 1) / a.turns;
+    const int64_t kv_blocks = (int64_t)a.windows * a.head_groups * 2, blocks = kv_blocks + ((int64_t)rows * a.parts + 3) / 4;
+    if (blocks > 0x7fffffff) return fail(BX_EUNSUPPORTED, "qkv_append_q8: too many rows and heads");
+    a.kv_blocks = (unsigned)kv_blocks;
+    hipStream_t st = as_stream(stream);
+    auto run = [&](auto hdc) {
+        constexpr int HD = decltype(hdc)::value;
+        if (page == 16) qkv_append_kernel<HD, 1><<<(unsigned)blocks, 256, 0, st>>>(a);
+        else if (page == 32) qkv_append_kernel<HD, 2><<<(unsigned)blocks, 256, 0, st>>>(a);
+        else if (page == 64) qkv_append_kernel<HD, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
+        else qkv_append_kernel<HD, 8><<<(unsigned)blocks, 256, 0, st>>>(a);
+    };
+    if (hd == 64) run(std::integral_constant<int, 64>{});
+    else if (hd == 128) run(std::integral_constant<int, 128>{});
+    else run(std::integral_constant<int, 256>{});
+    return launch_check("qkv_append_q8");
 }
 
 int bx_kv_read_q8_f16(const int64_t* slots, int rows, int n_kv, int hd, int page, int n_pages, const int8_t* Kc,

@@ -404,6 +404,67 @@ int bx_attention_paged_q8_f16(const uint16_t* q, int64_t q_stride, int rows, con
                               const float* v_scale, int n_q, int n_kv, int hd, int window, uint16_t* out,
                               int64_t out_stride, void* ws, size_t ws_bytes, void* stream);
 
+/* Requests that begin with the same text hold its keys once: request r may come
+ * behind the first keys of another request, parent[r].  Its own pages, length and
+ * block table then hold what comes after them (bx_kv_plan lays these out as always;
+ * the parent is a request like any other, with new rows or none).
+ *
+ * One step with shared prefixes: bx_kv_plan, bx_prefix_plan, then per layer
+ * bx_qkv_append_q8_f16 and bx_attention_prefix_q8_f16. */
+
+/* Positions and groups of a step's rows, from the plan's starts, lens and positions
+ * (pos_in), of n_req (<= 4096) requests.  Request r shares s = min(shared_lens[r],
+ * lens[parent[r]]) keys, the first of parent[r]'s own; 0 where parent[r] names no
+ * other request (negative, n_req or more, r) or shared_lens[r] is not positive.
+ * (A parent's own parent is not followed.)  For the max_rows rows:
+ *   pos[i] = pos_in[i] + s of its request (negative ones stay as they are);
+ *   shared[i] = s, 0 behind the last row;
+ *   order: the rows that share any keys, by parent, then by row; -1 behind them;
+ *   groups[k] (n_req): the parents of such rows, ascending, -1 behind them;
+ *   group_starts[k] (n_req + 1): where the rows of groups[k] begin in order; the
+ *   number of such rows behind them.
+ * pos may be pos_in (the plan's positions are then gone: once a step).  No other
+ * output may lie over an input or another output. */
+int bx_prefix_plan(const int32_t* parent, const int32_t* shared_lens, const int32_t* starts, const int32_t* lens,
+                   int n_req, const int32_t* pos_in, int32_t* pos, int32_t* shared, int32_t* order, int max_rows,
+                   int32_t* groups, int32_t* group_starts, void* stream);
+
+/* q, k and v of a step's rows as the projections leave them (rows apart by their
+ * strides; q n_q heads, k and v n_kv heads of hd) in one pass: RMSNorm of every q
+ * and k head with q_gain / k_gain (hd values; both null: none), the rotation of the
+ * pairs (2 i, 2 i + 1) by row pos[i] of the FP32 tables (tab_rows, hd / 2), in FP32
+ * with one rounding to FP16; q heads to q_out (may be q, at the same stride), K and
+ * V rows into the pages as bx_kv_append_q8_f16 puts FP16 rows there.  A row whose
+ * position lies outside the table leaves q_out as it is and enters the pages with
+ * K = 0; one whose slot lies outside the pool enters no page. */
+int bx_qkv_append_q8_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                         int64_t v_stride, int rows, int n_q, int n_kv, int hd, const uint16_t* q_gain,
+                         const uint16_t* k_gain, float eps, const int32_t* pos, const float* cos_tab,
+                         const float* sin_tab, int tab_rows, const int64_t* slots, int page, int n_pages, int8_t* Kc,
+                         int8_t* Vc, float* k_scale, float* v_scale, uint16_t* q_out, int64_t q_out_stride, void* stream);
+
+/* bx_attention_paged_q8_f16 for a step with shared prefixes: a row of request r
+ * attends the first shared[row] keys of its group's request, then r's own keys up to
+ * its own position; with a window, the last `window` of these.  Shared keys are read
+ * once for 128 / (n_q / n_kv) rows of a group.  starts, lens, table and the cache as there
+ * (own keys); pos, shared, order, groups and group_starts as bx_prefix_plan writes them.
+ * max_new and max_len (own keys) as there; max_groups >= the number of groups (rows
+ * of groups behind it may be left as they are); max_shared (about the most shared keys)
+ * shapes the launch.  The weights of shared keys enter the product with V as those of long chunks
+ * do; everything else as there.
+ * ws: bx_attention_prefix_q8_workspace_bytes(...) bytes with the same arguments (a
+ * workspace for several shapes: the largest), 16-byte aligned, its first 512 KB zeroed
+ * once before the first use; calls sharing one must not overlap. */
+size_t bx_attention_prefix_q8_workspace_bytes(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len,
+                                              int max_groups, int max_shared);
+int bx_attention_prefix_q8_f16(const uint16_t* q, int64_t q_stride, int rows, const int32_t* starts, const int32_t* lens,
+                               int n_req, int max_new, int max_len, const int32_t* pos, const int32_t* shared,
+                               const int32_t* order, const int32_t* groups, const int32_t* group_starts, int max_groups,
+                               int max_shared, const int32_t* table, int max_blocks, int page, int n_pages,
+                               const int8_t* Kc, const int8_t* Vc, const float* k_scale, const float* v_scale, int n_q,
+                               int n_kv, int hd, int window, uint16_t* out, int64_t out_stride, void* ws, size_t ws_bytes,
+                               void* stream);
+
 /* ------------------------------------------------------------ decode step */
 
 /* Fused single-token decode kernels (the captured step of
