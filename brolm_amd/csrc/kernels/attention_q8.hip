@@ -58,6 +58,9 @@ constexpr int64_t kQaRecBytes = 128 << 20;   // records of either kind of tile, 
 constexpr int kQaNarrowReq = 256;    // requests whose narrow tiles a wavefront counts in four steps
 constexpr int kQaNarrowCols = 64;    // columns a request up to which narrow tiles serve any batch
 constexpr int64_t kQaNarrowWork = (int64_t)1 << 27;   // bytes of K that they read, for more columns
+constexpr int kQsMaxSplits = 63;   // of shared keys; with the own ones a lane each in the join
+constexpr int kQsLeast = 4;        // tiles of 64 shared keys a part
+constexpr int64_t kQsWideWork = (int64_t)1 << 25;   // pairs of a row's head and a shared key from which wide tiles pay
 constexpr int kQaWords = 32768;   // arrival counters of either kind of tile
 
 struct QaArgs {
@@ -322,12 +325,13 @@ struct QaTile {
     bool ok;
 };
 
-// NT: rows by streaming loads (below, at the launch).
+// NT: rows by streaming loads (below, at the launch).  tid: the thread of the 256 (a workgroup of
+// qs_wide_kernel is two of them).
 template <int HD, bool NT, class A>
-__device__ __forceinline__ void qa_tile(const A& a, unsigned block, unsigned char* smem) {
+__device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block, unsigned char* smem) {
     constexpr int NC = HD / 64, NJ = HD / 16;
     constexpr bool PART = std::is_same_v<A, QsArgs>;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
     // ---- block -> (tile of 16 columns, split, KV head)
@@ -574,7 +578,7 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned block, unsigned cha
     __syncthreads();
     uint64_t* const word = a.cnt + tile * a.n_kv + g;
     uint32_t* const last = reinterpret_cast<uint32_t*>(smem);
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         *last = tagged_arrive(word, a.tag) == (uint32_t)T ? 1u : 0u;
         if (*last) __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -664,11 +668,12 @@ __device__ __forceinline__ int row16_of(int v, F&& op) {
 // SHARED: columns are the rows that share the keys of one request (a group of the plan), 128
 // of them a tile, each with its own last key; what each part gave is left for the join.
 template <int HD, bool SHARED, class A>
-__device__ __forceinline__ void qa_rows_tile(const A& a, unsigned block, unsigned blocks, unsigned char* smem) {
+__device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned block, unsigned blocks,
+                                             unsigned char* smem) {
     using S = QrShape<HD>;
     constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI, KB = HD > 128 ? 1 : 2;
     constexpr bool PART = std::is_same_v<A, QsArgs>;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
     // ---- block -> (column tile, split, KV head): the last tiles first, they see the
@@ -774,7 +779,7 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned block, unsigne
     // and of head dim .. (V) of the 16 keys grp = thread / HD + i (256 / HD)
     const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
     const int last_block = max(0, (kend - 1) >> a.pshift);
-    const int in = threadIdx.x % HD, grp0 = __builtin_amdgcn_readfirstlane(threadIdx.x / HD);
+    const int in = tid % HD, grp0 = __builtin_amdgcn_readfirstlane(tid / HD);
     const int kkey = in / (HD / 16), kunit = in % (HD / 16);   // K: key of the 16, piece of the row
     u4v kx[NI], vx[NI];
     // page ids a turn before the rows that they lead to, and those of the lane's 16 keys
@@ -992,7 +997,7 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned block, unsigne
     __syncthreads();
     uint64_t* const word = a.cnt + tile * a.n_kv + g;
     uint32_t* const last = reinterpret_cast<uint32_t*>(smem);   // (the tiles are done with)
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         *last = tagged_arrive(word, a.tag) == (uint32_t)T ? 1u : 0u;
         if (*last) __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -1034,7 +1039,7 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned block, unsigne
 template <int HD, bool NT>
 __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
-    qa_tile<HD, NT>(a, blockIdx.x, smem);
+    qa_tile<HD, NT>(a, threadIdx.x, blockIdx.x, smem);
 }
 
 // Both kinds of tiles in one launch, the long ones first: decode rows fill the CUs that
@@ -1042,21 +1047,463 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
 template <int HD>
 __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_both_kernel(QaArgs rows, QaArgs a, unsigned row_blocks) {
     extern __shared__ __align__(16) unsigned char smem[];
-    if (blockIdx.x < row_blocks) qa_rows_tile<HD, false>(rows, blockIdx.x, row_blocks, smem);
-    else qa_tile<HD, false>(a, blockIdx.x - row_blocks, smem);
+    if (blockIdx.x < row_blocks) qa_rows_tile<HD, false>(rows, threadIdx.x, blockIdx.x, row_blocks, smem);
+    else qa_tile<HD, false>(a, threadIdx.x, blockIdx.x - row_blocks, smem);
 }
 
 // A step with shared prefixes in one launch: tiles of the shared keys, which are the longest,
-// then those of the own keys as above.
+// then those of the own keys as above.  Here the shared ones in tiles of 128 columns, as those of chunks.
 template <int HD>
 __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qs_kernel(QsArgs shared, QsArgs rows, QsArgs a,
                                                                          unsigned shared_blocks, unsigned row_blocks) {
     extern __shared__ __align__(16) unsigned char smem[];
     unsigned b = blockIdx.x;
-    if (b < shared_blocks) return qa_rows_tile<HD, true>(shared, b, shared_blocks, smem);
+    if (b < shared_blocks) return qa_rows_tile<HD, true>(shared, threadIdx.x, b, shared_blocks, smem);
     b -= shared_blocks;
-    if (b < row_blocks) return qa_rows_tile<HD, false>(rows, b, row_blocks, smem);
-    qa_tile<HD, false>(a, b - row_blocks, smem);
+    if (b < row_blocks) return qa_rows_tile<HD, false>(rows, threadIdx.x, b, row_blocks, smem);
+    qa_tile<HD, false>(a, threadIdx.x, b - row_blocks, smem);
+}
+
+// Shared keys, heads of 64 and 128: a workgroup of eight wavefronts takes 256 columns of a group,
+// a wavefront 32, and walks tiles of 64 keys (SOLO: 128 columns at most; the wavefronts 0 .. 3
+// take the first 32 keys of a tile and 4 .. 7 the others, and join at the end).  The wavefronts w
+// and w + 4, which share a SIMD, work half a tile apart: while one multiplies (P V of a tile
+// and Q K^T of the next on v_mfma_f32_32x32x16_f16, operands from LDS), the other has the vector
+// unit for its softmax, and a barrier hands over.  Every thread converts its share of the tile after
+// that to FP16 integers, once for all columns, between its matrix instructions; K has two
+// buffers and V three.
+// The rows of K are permuted in the operand so that a lane's 16 products of a fragment are keys 8
+// h .. + 7 and 16 + 8 h .. + 7 (h = lane / 32): P is an operand as it stands.
+template <int HD>
+struct QsShape {
+    static constexpr int kTile = 64 * HD * 2;          // bytes of a K or V tile
+    // K, V, the scales of three tiles, and as much room for the threads that store none
+    static constexpr int kV = 2 * kTile, kScales = 5 * kTile, kNone = kScales + 3 * 128, kLds = kNone + 512 * 32 + 3 * 128;
+    // 16-byte chunk c of key k sits at c ^ kswz(k), of head dim d at c ^ vswz(d): 16 keys or head dims
+    // of a chunk cover the 64 banks
+    static __device__ __forceinline__ int kswz(int k) { return HD == 128 ? k & 15 : (k >> 1) & 7; }
+    static __device__ __forceinline__ int vswz(int d) { return (d >> 1) & 7; }
+};
+
+typedef float qa_f16v __attribute__((ext_vector_type(16)));
+
+template <int HD, bool SOLO>
+__device__ __forceinline__ void qs_tile(const QsArgs& a, int r, int g, int s, int64_t c0, int64_t ncol, int row0,
+                                        unsigned char* smem) {
+    using S = QsShape<HD>;
+    constexpr int ND = HD / 16, NJ = HD / 32, NK = SOLO ? 1 : 2, NU = 2 * NK;   // steps along hd; fragments of hd, of keys; of 16 keys
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lc = lane & 31, lh = lane >> 5, G = a.G, page = 1 << a.pshift;
+    const int kf0 = SOLO ? wave >> 2 : 0;   // the first fragment of 32 keys
+    const int len = (int)min((int64_t)max(0, a.lens[r]), (int64_t)a.max_blocks << a.pshift);
+
+    // ---- this wavefront's columns; they see keys plow .. plast
+    const int64_t w0 = c0 + 32 * (SOLO ? wave & 3 : wave), c = w0 + lc;
+    const bool works = w0 < ncol;
+    bool real = c < ncol;
+    const int64_t cc = real ? c : c0;
+    const int head = g * G + (int)(cc % G);
+    int row = a.order[row0 + (int)(cc / G)];
+    if (row < 0 || row >= a.rows) {
+        real = false;
+        row = 0;
+    }
+    const int plast = real ? min(a.shared[row], len) - 1 : -1, plow = first_key(a.pos[row], a.window);
+    qa_h8 qf[ND];
+    {
+        const uint16_t* const q = a.q + (int64_t)row * a.q_stride + (int64_t)head * HD + 8 * lh;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) qf[d] = __builtin_bit_cast(qa_h8, (u4v)*reinterpret_cast<const qa_any16*>(q + 16 * d));
+    }
+    constexpr int kMost = 0x7fffffff;
+    auto over32 = [](int v, auto op) {   // over the wavefront's 32 columns
+        v = row16_of(v, op);
+        return __builtin_amdgcn_readfirstlane(op(v, __shfl_xor(v, 16)));
+    };
+    auto mn = [](int x, int y) { return min(x, y); };
+    auto mx = [](int x, int y) { return max(x, y); };
+    const int low_min = over32(real ? plow : kMost, mn), low_max = over32(real ? plow : 0, mx);
+    const int last_min = over32(real ? plast : kMost, mn), last_max = over32(plast, mx);
+    int* const ends = reinterpret_cast<int*>(smem);
+    if (lane == 0) {
+        ends[wave] = low_min;
+        ends[8 + wave] = last_max;
+    }
+    __syncthreads();
+    int kend = -1, k64 = kMost;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        kend = max(kend, ends[8 + w]);
+        k64 = min(k64, ends[w]);
+    }
+    kend = __builtin_amdgcn_readfirstlane(kend + 1);
+    k64 = __builtin_amdgcn_readfirstlane(min(k64, kend) / 64);
+    __syncthreads();   // the tiles go there
+    const int n64 = (kend + 63) / 64 - k64;
+    const int ku = max(kQsLeast, (n64 + a.S - 1) / a.S), T = max(1, (n64 + ku - 1) / ku);
+    if (s >= T) return;
+    k64 += s * ku;
+    const int n = max(0, min(ku, n64 - s * ku));   // this part's tiles
+
+    // ---- tiles through registers: a thread's piece is 16 codes of a key (K) and of a head dim (V)
+    // of 16 keys; heads of 64 have half as many, one to a thread.  The 16 keys, and so the page,
+    // are the wavefront's: its id comes a turn ahead (in a vector register, made scalar where it is
+    // used: a scalar one would be waited for at once)
+    constexpr bool BOTH = HD == 128;
+    const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
+    const int last_block = max(0, (kend - 1) >> a.pshift);
+    const int in = tid % HD, vgrp = (tid / HD) & 3, grp = __builtin_amdgcn_readfirstlane(vgrp);
+    const bool is_v = !BOTH && __builtin_amdgcn_readfirstlane(tid / HD) >= 4;   // (heads of 64)
+    const int kkey = in / (HD / 16), kunit = in % (HD / 16), key16 = 16 * grp + kkey;
+    auto page_at = [&](int i) {
+        return *gptr<int32_t>(trow + min(((k64 + i) * 64 + 16 * vgrp) >> a.pshift, last_block));
+    };
+    const uint32_t page_bytes = (uint32_t)(a.n_kv * page * HD);   // of all heads; below 2^31
+    const int8_t* const kg = a.Kc + (int64_t)g * page * HD + kkey * HD + 16 * kunit;
+    const int8_t* const vg = a.Vc + (int64_t)g * page * HD + in * page;
+    // the two 16-byte chunks of a converted piece lie 16 bytes apart, the first at an even or odd place
+    const int kdst = key16 * HD * 2 + (((2 * kunit) ^ S::kswz(key16)) << 4), vdst = in * 128 + (((2 * grp) ^ S::vswz(in)) << 4);
+    u4v xk, xv;      // the pieces of the tile after next
+    int id;          // the page of the one after that
+    bool id_ok;      // of the tile that the pieces are of, as `sk`, `sv`
+    float sk = 0.f, sv = 0.f;
+    const int sdst = in == 0 && !is_v ? S::kScales + 32 * grp : S::kNone + 32 * tid;
+    // Pieces of work of a few instructions, one at most between two matrix instructions (a product
+    // takes 32 cycles of the matrix unit, an instruction 4 to issue): they store the pieces at hand as
+    // tile i + 1 (V and scales in slot v2) and ask for those of tile i + 2 and the page after that.
+    // What the softmax takes of 16 keys is their K scale times log2(e) / sqrt(hd); of the V scale as P
+    // carries it (QaScale) the base-2 logarithm + kQaReserve and the inverse; 1 where the page is
+    // none, 2 where its V scale is not finite; and that.
+    constexpr int kWork = 16;
+    uint32_t t0 = 0u, t1 = 0u;
+    qa_f4 xs{0.f, 0.f, 0.f, 0.f};
+    float rs = 1.f;
+    int sid = 0, key = 0;
+    int64_t hp = 0;
+    auto work = [&](int i, int v2, auto kc) {
+        constexpr int k = decltype(kc)::value;
+        if constexpr (k < 8) {
+            constexpr bool V = k >= 4;
+            constexpr int e = k / 2 % 2;
+            if constexpr (BOTH || !V) {
+                const u4v& w = V ? xv : xk;
+                if constexpr (k % 2 == 0) {
+                    codes_f16(w[2 * e], t0, t1);
+                } else {
+                    uint32_t t2, t3;
+                    codes_f16(w[2 * e + 1], t2, t3);
+                    const int ko = ((i + 1) & 1) * S::kTile + kdst, vo = S::kV + v2 * S::kTile + vdst;
+                    *reinterpret_cast<u4v*>(smem + ((BOTH ? (V ? vo : ko) : (is_v ? vo : ko)) ^ (16 * e))) = u4v{t0, t1, t2, t3};
+                }
+            }
+        } else if constexpr (k == 8) {
+            const bool fin = sv < INFINITY;
+            rs = fin ? fminf(fmaxf(sv, kQaLeastScale), kQaMostScale) : 1.f;
+            xs[3] = !id_ok ? 1.f : fin ? 0.f : 2.f;
+        } else if constexpr (k == 9) {
+            xs[0] = sk * (1.4426950408889634f / sqrtf((float)HD));
+            xs[1] = __builtin_amdgcn_logf(rs) + (float)kQaReserve;
+            xs[2] = __builtin_amdgcn_rcpf(rs);
+            unsigned char* const at = smem + sdst + 128 * v2;
+            *reinterpret_cast<qa_f4*>(at) = xs;
+            reinterpret_cast<float*>(at)[4] = sv;
+        } else if constexpr (k == 10) {
+            sid = __builtin_amdgcn_readfirstlane(id);
+            id_ok = sid >= 0 && sid < a.n_pages;
+            sid = id_ok ? sid : 0;
+        } else if constexpr (k == 11) {
+            key = ((k64 + i + 2) * 64 + 16 * grp) & (page - 1);
+            hp = (int64_t)((uint64_t)(uint32_t)sid * page_bytes);
+        } else if constexpr (k == 12) {
+            if constexpr (BOTH) xk = *gptr<u4v>(kg + hp + key * HD);
+            else xk = *gptr<u4v>((is_v ? vg + key : kg + key * HD) + hp);
+        } else if constexpr (k == 13) {
+            if constexpr (BOTH) xv = *gptr<u4v>(vg + hp + key);
+        } else if constexpr (k == 14) {
+            const int64_t at = (int64_t)sid * a.n_kv + g;
+            sk = *gptr<float>(a.ks + at);
+            sv = *gptr<float>(a.vs + at);
+        } else {
+            id = page_at(i + 3);
+        }
+    };
+
+    qa_f16v o[NJ], y[NK];
+    qa_h8 pb[NU];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
+    // ---- P V of tile i - 1 (V in slot v0), Q K^T of tile i, and the work above: a matrix
+    // instruction a step, whose operand from LDS was asked for kAhead steps before
+    constexpr int kAhead = 4;
+    const int krow = 16 * (lc >> 4) + 8 * ((lc >> 2) & 1) + 4 * ((lc >> 3) & 1) + (lc & 3);   // of 32
+    const int ka = (32 * kf0 + krow) * HD * 2, ksw = S::kswz(krow);   // (kswz has no bit above 15 of the key)
+    const int va = lc * 128, vsw = S::vswz(lc);
+    qa_h8 f[kAhead + 1];
+    // the first operands, V's, while the vector unit is at work
+    auto ahead = [&](int v0) {
+        const unsigned char* const vt = smem + S::kV + v0 * S::kTile + va;
+        static_for<kAhead>([&](auto kc) {
+            constexpr int j = decltype(kc)::value % NJ, u = decltype(kc)::value / NJ;
+            f[decltype(kc)::value] = *reinterpret_cast<const qa_h8*>(vt + 32 * j * 128 + (((4 * kf0 + 2 * u + lh) ^ vsw) << 4));
+        });
+    };
+    auto multiply = [&](auto qkc, int i, int v0, int v2) {   // (behind the last tile P V alone)
+        constexpr bool QK = decltype(qkc)::value;
+        constexpr int NP = NJ * NU, N = NP + (QK ? ND * NK : 0);
+        const unsigned char* const vt = smem + S::kV + v0 * S::kTile + va;
+        const unsigned char* const kt = smem + (i & 1) * S::kTile + ka;
+        auto read = [&](auto kc) {
+            constexpr int k = decltype(kc)::value;
+            if constexpr (k < NP) {   // fragment j of V^T, keys 16 u ..
+                constexpr int j = k % NJ, u = k / NJ;
+                f[k % (kAhead + 1)] = *reinterpret_cast<const qa_h8*>(vt + 32 * j * 128 + (((4 * kf0 + 2 * u + lh) ^ vsw) << 4));
+            } else if constexpr (k < N) {
+                constexpr int kf = (k - NP) % NK, d = (k - NP) / NK;
+                f[k % (kAhead + 1)] = *reinterpret_cast<const qa_h8*>(kt + 32 * kf * HD * 2 + (((2 * d + lh) ^ ksw) << 4));
+            }
+        };
+        static_for<N>([&](auto kc) {
+            constexpr int k = decltype(kc)::value;
+            read(std::integral_constant<int, k + kAhead>{});
+            if constexpr (k < NP) {
+                constexpr int j = k % NJ, u = k / NJ;
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k % (kAhead + 1)], pb[u], o[j], 0, 0, 0);
+            } else {
+                constexpr int kf = (k - NP) % NK, d = (k - NP) / NK;
+                if constexpr (d == 0) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) y[kf][e] = 0.f;
+                }
+                y[kf] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k % (kAhead + 1)], qf[d], y[kf], 0, 0, 0);
+            }
+            if constexpr (QK)
+                static_for<kWork>([&](auto wc) {
+                    if constexpr (decltype(wc)::value * N / kWork == k) work(i, v2, wc);
+                });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto only_work = [&](int i, int v2) { static_for<kWork>([&](auto wc) { work(i, v2, wc); }); };
+    // ---- the softmax step of qa_softmax (there: why P is what it is), with l as the sum of the P that
+    // the product takes
+    auto weigh = [&](int i, int slot) {
+        const float* const sc = reinterpret_cast<const float*>(smem + S::kScales) + (4 * slot + 2 * kf0) * 8;
+        const int k0 = (k64 + i) * 64 + 32 * kf0;
+        qa_f4 x[NU];
+        float flags = 0.f;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            x[u] = *reinterpret_cast<const qa_f4*>(sc + 8 * u);
+            flags += x[u][3];
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const float nr = x[u][1] - shift;
+#pragma unroll
+            for (int e = 8 * (u % 2); e < 8 * (u % 2) + 8; ++e) y[u / 2][e] = __builtin_fmaf(y[u / 2][e], x[u][0], nr);
+        }
+        const bool odd = __any(flags != 0.f);
+        // keys behind a column's last, before its first (windows), and of pages that are none: a column
+        // that forks off early has every later tile masked
+        auto hide = [&](auto what) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (what(u, 16 * u + e)) y[u / 2][8 * (u % 2) + e] = -INFINITY;
+        };
+        if (k0 + 32 * NK - 1 > last_min) {
+            const int last = plast - k0 - 8 * lh;
+            hide([&](int, int z) { return z > last; });
+        }
+        if (k0 < low_max) {
+            const int first = plow - k0 - 8 * lh;
+            hide([&](int, int z) { return z < first; });
+        }
+        if (odd) hide([&](int u, int) { return x[u][3] == 1.f; });
+        float top = y[0][0];
+#pragma unroll
+        for (int z = 1; z + 1 < 16 * NK; z += 2)
+            top = fmaxf(fmaxf(top, y[z / 16][z % 16]), y[(z + 1) / 16][(z + 1) % 16]);
+        top = fmaxf(top, y[NK - 1][15]);
+        if (__any(top > (m == -INFINITY ? -INFINITY : (float)(kQaReserve + kQaLazy)))) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float((uint32_t)sw[0]), __uint_as_float((uint32_t)sw[1]));
+            const float now = fmaxf(m, top + shift - (float)kQaReserve);
+            const float d = now == m ? 0.f : shift - now, al = now == m ? 1.f : __builtin_amdgcn_exp2f(m - now);
+            l *= al;
+            m = now;
+#pragma unroll
+            for (int kf = 0; kf < NK; ++kf)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[kf][e] += d;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[j][e] *= al;
+        }
+        const qa_h2 one{(_Float16)1.f, (_Float16)1.f};
+        if (!odd) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                float ls = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const qa_h2 p{(_Float16)__builtin_amdgcn_exp2f(y[u / 2][8 * (u % 2) + e]),
+                                  (_Float16)__builtin_amdgcn_exp2f(y[u / 2][8 * (u % 2) + e + 1])};
+                    ls = __builtin_amdgcn_fdot2(p, one, ls, false);
+                    pb[u][e] = p.x;
+                    pb[u][e + 1] = p.y;
+                }
+                l = __builtin_fmaf(ls, x[u][2], l);
+            }
+        } else {   // a page without a finite V scale: a hidden key weighs nothing whatever that is
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float z = y[u / 2][8 * (u % 2) + e];
+                    asm volatile("" : "+v"(z));   // (or both branches' exponentials are formed before them)
+                    const float p = __builtin_amdgcn_exp2f(z);
+                    l = __builtin_fmaf(p, x[u][2], l);
+                    pb[u][e] = (_Float16)(x[u][3] != 2.f ? p : z == -INFINITY ? 0.f : p * sc[8 * u + 4]);
+                }
+        }
+    };
+    // LDS stores done, loads from memory may be under way
+    auto hand_over = [&] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (n > 0) {
+        id = page_at(0);
+        static_for<5>([&](auto wc) { work(-2, 0, std::integral_constant<int, 10 + decltype(wc)::value>{}); });
+        id = page_at(1);
+        only_work(-1, 0);   // the first tile stored, the second asked for
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pb[u][e] = (_Float16)0.f;
+        hand_over();
+        ahead(0);
+        if (wave >= 4) hand_over();   // half a tile behind
+        // slots of V of the tile before (for the first: its own, with P = 0), this one and the next
+        int v0 = 0, v1 = 0, v2 = 1;
+        auto next = [&] {
+            v0 = v1;
+            v1 = v2;
+            v2 = v2 == 2 ? 0 : v2 + 1;
+        };
+        if (works) {
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                __builtin_amdgcn_s_setprio(2);   // few instructions, which the other's many would hold up
+                multiply(std::true_type{}, i, v0, v2);
+                __builtin_amdgcn_s_setprio(0);
+                hand_over();
+                weigh(i, v1);
+                ahead(v1);
+                hand_over();
+                next();
+            }
+            multiply(std::false_type{}, n, v0, v2);
+        } else {   // no columns: the conversions alone
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                only_work(i, v2);
+                hand_over();
+                hand_over();
+                next();
+            }
+        }
+        if (wave < 4) hand_over();
+    }
+    {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float((uint32_t)sw[0]) + __uint_as_float((uint32_t)sw[1]);
+    }
+    if constexpr (SOLO) {   // the other half of the keys
+        qa_f4* const so = reinterpret_cast<qa_f4*>(smem) + ((wave & 3) * (4 * NJ + 1)) * 64 + lane;
+        __syncthreads();
+        if (wave >= 4) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) so[(4 * j + q) * 64] = qa_f4{o[j][4 * q], o[j][4 * q + 1], o[j][4 * q + 2], o[j][4 * q + 3]};
+            so[4 * NJ * 64] = qa_f4{m, l, 0.f, 0.f};
+        }
+        __syncthreads();
+        if (wave >= 4) return;
+        const qa_f4 ml = so[4 * NJ * 64];
+        const float M = fmaxf(m, ml[0]);
+        const float wa = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+        const float wb = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - M);
+        m = M;
+        l = wa * l + wb * ml[1];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const qa_f4 x = so[(4 * j + q) * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][4 * q + e] = wa * o[j][4 * q + e] + wb * x[e];
+            }
+    }
+    if (!works || !real) return;
+    // lane: column lane % 32, head dims 32 j + 8 q + 4 h ..
+    const int64_t n_q = (int64_t)a.n_kv * G, at = ((int64_t)(1 + s) * a.rows + row) * n_q + head;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<qa_f4*>(a.part + at * HD + 32 * j + 8 * q + 4 * lh) =
+                qa_f4{o[j][4 * q], o[j][4 * q + 1], o[j][4 * q + 2], o[j][4 * q + 3]};
+    if (lh == 0) {
+        *reinterpret_cast<f2v*>(a.part_ml + 2 * at) = f2v{m, l};
+        if (s == 0) a.part_n[row * n_q + head] = T;
+    }
+}
+
+template <int HD>
+struct QsWide {   // a workgroup's LDS: a tile of shared keys, or two workgroups' of own ones
+    static constexpr int kHalf = std::max(HD / 16 * 4096 + 512, 2 * QrShape<HD>::kBuf);
+    static constexpr int kLds = std::max(2 * kHalf, QsShape<HD>::kLds);
+};
+
+// The same with the shared ones in tiles of 256 columns, and two tiles of own ones to a workgroup
+// (a barrier waits for the wavefronts of both that have not ended).
+template <int HD>
+__global__ __launch_bounds__(2 * kQaThreads, 2) void qs_wide_kernel(QsArgs shared, QsArgs rows, QsArgs a, unsigned shared_blocks,
+                                                                   unsigned row_blocks, unsigned blocks) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    if (blockIdx.x < shared_blocks) {
+        // block -> (tile, part, KV head): a head's tiles on one XCD
+        const unsigned rest = blockIdx.x / (unsigned)a.n_kv;
+        const int g = (int)(blockIdx.x % (unsigned)a.n_kv), s = (int)(rest % (unsigned)shared.S);
+        const int64_t tile = rest / (unsigned)shared.S;
+        int k = 0, hi = shared.max_groups;
+        while (hi - k > 1) {
+            const int mid = (k + hi) >> 1;
+            if ((int64_t)shared.group_starts[mid] * a.G / 256 + mid <= tile) k = mid;
+            else hi = mid;
+        }
+        const int row0 = shared.group_starts[k], n_new = shared.group_starts[k + 1] - row0, r = shared.groups[k];
+        const int64_t ti = tile - ((int64_t)row0 * a.G / 256 + k), ncol = (int64_t)n_new * a.G, c0 = 256 * ti;
+        if (row0 < 0 || n_new <= 0 || row0 > a.rows - n_new || ti < 0 || c0 >= ncol || r < 0 || r >= a.n_req) return;
+        if (ncol - c0 > 128) qs_tile<HD, false>(shared, r, g, s, c0, ncol, row0, smem);
+        else qs_tile<HD, true>(shared, r, g, s, c0, ncol, row0, smem);
+        return;
+    }
+    const unsigned half = __builtin_amdgcn_readfirstlane(threadIdx.x / kQaThreads), tid = threadIdx.x % kQaThreads;
+    const unsigned b = 2 * (blockIdx.x - shared_blocks) + half;
+    unsigned char* const own = smem + half * QsWide<HD>::kHalf;
+    if (b < row_blocks) qa_rows_tile<HD, false>(rows, tid, b, row_blocks, own);
+    else if (b - row_blocks < blocks) qa_tile<HD, false>(a, tid, b - row_blocks, own);
 }
 
 // Joins what the own keys and the parts of the shared ones gave, a wavefront to a row and
@@ -1187,12 +1634,11 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     return p;
 }
 
-// A step with shared prefixes: the own keys as above, the shared ones in `tiles` of 128 columns
-// at most, the keys of each over S workgroups.
-constexpr int kQsMaxSplits = 63;   // and the own keys: a lane each in the join
-
+// A step with shared prefixes: the own keys as above, the shared ones in `tiles` of 256 (wide) or 128
+// columns at most, the keys of each over S workgroups.
 struct QsPlan {
     QaPlan own;
+    bool wide;
     int groups, S;
     int64_t tiles;
     size_t part_bytes, ml_bytes, n_bytes;
@@ -1202,12 +1648,31 @@ struct QsPlan {
 QsPlan qs_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int max_len, int max_groups, int max_shared) {
     QsPlan p{};
     p.own = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
-    const int64_t G = n_q / n_kv, cus = num_cus(), slots = hd > 128 ? cus : 2 * cus;
     p.groups = std::min({max_groups, n_req, rows});
-    p.tiles = (int64_t)rows * G / 128 + p.groups;
-    const int64_t likely = (((int64_t)rows * G + 127) / 128 + p.groups - 1) * n_kv, each = (int64_t)rows * n_q * hd * 4;
+    const int64_t G = n_q / n_kv, cus = num_cus();
+    // Tiles of 256 columns do more products for every operand from LDS and code converted, those of 128
+    // leave more workgroups and share the chip better with the own keys.  32 / 8 heads of 128,
+    // wide against 128: 1,640 rows (8 chunks and 32 single tokens) on prefixes of 9,000 and 6,750 keys
+    // 289 us and 370; 114 rows on 30,000 119 and 128; 480 rows (2 chunks) on 9,000 124 and 136; 130
+    // rows on 6,000 74 and 74; 36 on 20,000 56 and 54; 57 on 6,000 48 and 43; 45 rows of 24 / 8
+    // heads of 64 on seven of 2,900 to 5,000 43 and 34.
+    p.wide = hd <= 128 && (int64_t)rows * G > 128 * (int64_t)p.groups && (int64_t)rows * n_q * max_shared > kQsWideWork;
+    const int64_t cols = p.wide ? 256 : 128, slots = p.wide || hd > 128 ? cus : 2 * cus;
+    p.tiles = (int64_t)rows * G / cols + p.groups;
+    const int64_t likely = (((int64_t)rows * G + cols - 1) / cols + p.groups - 1) * n_kv, each = (int64_t)rows * n_q * hd * 4;
     const int64_t cap = std::max<int64_t>(1, std::min<int64_t>({((int64_t)max_shared + 255) / 256, kQsMaxSplits, kQaRecBytes / each}));
-    p.S = (int)std::max<int64_t>(1, std::min(slots / likely, cap));
+    // Rounds of workgroups that take as long as their tiles (2 us each) and two more to begin, and what they
+    // leave, which is written and read (5 TB/s): the least of that.
+    p.S = 1;
+    double least = 1e30;
+    for (int64_t n = 1; n <= cap; ++n) {
+        const double t = (double)((likely * n + slots - 1) / slots) * 2.0 * (std::max<double>(kQsLeast, max_shared / 64.0 / n) + 2.0) +
+                         (double)each * n * 0.4e-6;
+        if (t < 0.98 * least) {
+            least = t;
+            p.S = (int)n;
+        }
+    }
     auto up = [](int64_t x) { return ((size_t)x + 255) / 256 * 256; };
     p.part_bytes = up(each * (1 + p.S));
     p.ml_bytes = up((int64_t)rows * n_q * 8 * (1 + p.S));
@@ -1322,6 +1787,7 @@ int bx_attention_prefix_q8_f16(const uint16_t* q, int64_t q_stride, int rows, co
         return fail(BX_EINVAL, "attention_prefix_q8: row stride below n_q * head_dim");
     if ((int64_t)max_blocks * page > 0x7fffffff - 4095)   // the tiles asked for ahead lie below 2^31 too
         return fail(BX_EUNSUPPORTED, "attention_prefix_q8: more than 2^31 - 4096 tokens a request");
+    if ((int64_t)n_kv * page * hd > 0x7fffffff) return fail(BX_EUNSUPPORTED, "attention_prefix_q8: pages of 2^31 bytes and more");
     const QsPlan p = qs_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len, max_groups, max_shared);
     if (ws_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(ws) & 15))
         return fail(BX_EINVAL, "attention_prefix_q8: workspace too small or not 16-byte aligned");
@@ -1355,13 +1821,23 @@ int bx_attention_prefix_q8_f16(const uint16_t* q, int64_t q_stride, int rows, co
     hipStream_t st = as_stream(stream);
     auto run = [&](auto hdc) -> int {
         constexpr int HD = decltype(hdc)::value, lds = std::max(HD / 16 * 4096 + 512, 2 * QrShape<HD>::kBuf);
-        if constexpr (lds > 64 * 1024) {
-            static std::atomic<uint64_t> allowed{0};
-            if (int rc = allow_lds(allowed, reinterpret_cast<const void*>(&qs_kernel<HD>), lds, "attention_prefix_q8: LDS attribute"))
-                return rc;
+        static std::atomic<uint64_t> allowed[2];
+        if constexpr (HD <= 128) {
+            if (p.wide) {
+                constexpr int wlds = QsWide<HD>::kLds;
+                if (int rc = allow_lds(allowed[1], reinterpret_cast<const void*>(&qs_wide_kernel<HD>), wlds, "attention_prefix_q8: LDS attribute"))
+                    return rc;
+                qs_wide_kernel<HD><<<(unsigned)(sblocks + (rblocks + blocks + 1) / 2), 2 * kQaThreads, wlds, st>>>(
+                    as, ar, a, (unsigned)sblocks, (unsigned)rblocks, (unsigned)blocks);
+            }
         }
-        qs_kernel<HD><<<(unsigned)(sblocks + rblocks + blocks), kQaThreads, lds, st>>>(as, ar, a, (unsigned)sblocks,
-                                                                                      (unsigned)rblocks);
+        if (!p.wide) {
+            if constexpr (lds > 64 * 1024)
+                if (int rc = allow_lds(allowed[0], reinterpret_cast<const void*>(&qs_kernel<HD>), lds, "attention_prefix_q8: LDS attribute"))
+                    return rc;
+            qs_kernel<HD><<<(unsigned)(sblocks + rblocks + blocks), kQaThreads, lds, st>>>(as, ar, a, (unsigned)sblocks,
+                                                                                          (unsigned)rblocks);
+        }
         if (int rc = launch_check("attention_prefix_q8")) return rc;
         qs_join_kernel<HD><<<(unsigned)joins, kQaThreads, 0, st>>>(as);
         return launch_check("attention_prefix_q8: join");

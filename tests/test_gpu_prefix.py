@@ -327,6 +327,61 @@ def test_attention_prefix_chunks_of_large_batches(n_q, n_kv, hd, page, window):
           window, max_new=400, max_len=1 << 21, max_groups=5, max_shared=1 << 21)
 
 
+WIDE = [  # prefixes' lengths, requests, rows each, heads, kv heads, hd, page
+    ([700], 65, 1, 8, 2, 128, 64), ([700], 64, 1, 8, 2, 64, 16), ([300, 1000], 88, 1, 6, 2, 128, 16), ([513, 64], 50, 3, 16, 4, 64, 128),
+    ([90], 7, 40, 3, 3, 128, 32), ([2000], 33, 1, 16, 1, 128, 128), ([129], 260, 1, 1, 1, 64, 32)]
+
+
+@pytest.mark.parametrize("case", range(len(WIDE)))
+@pytest.mark.parametrize("window", [0, 77, 400])
+def test_attention_prefix_wide_tiles(case, window):
+    """Tiles of 256 columns, whole and with a half to 128 and less: a bound on the shared keys that
+    allows for far more work; forks everywhere, a third from the first tile."""
+    prefixes, requests, m, n_q, n_kv, hd, page = WIDE[case]
+    rng = np.random.default_rng(case * 5 + window)
+    k = len(prefixes)
+    parent = [-1] * k + [int(i % k) for i in range(requests)]
+    shared_lens = [0] * k + [int(rng.integers(1, 65)) if rng.random() < 0.3 else int(rng.integers(1, prefixes[p] + 1)) for p in parent[k:]]
+    lens = prefixes + [int(rng.integers(m, m + 20)) for _ in range(requests)]
+    # 2^25 pairs of a row's head and a shared key and more
+    _case(rng, lens, [0] * k + [m] * requests, parent, shared_lens, n_q, n_kv, hd, page, window, max_groups=k,
+          max_shared=(1 << 25) // (requests * m * n_q) + 1)
+
+
+@pytest.mark.parametrize("hd,rows", [(64, 140), (128, 150)])
+def test_attention_prefix_wide_tiles_long(hd, rows):
+    """Many tiles of keys to a workgroup, more than its buffers hold."""
+    rng = np.random.default_rng(rows)
+    lens, parent = [14500] + [3] * rows, [-1] + [0] * rows
+    shared_lens = [0] + [int(rng.choice([14500, 14399, 9000])) for _ in range(rows)]
+    _case(rng, lens, [0] + [1] * rows, parent, shared_lens, 16, 1, hd, 64)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_prefix_wide_tiles_of_odd_pages(hd):
+    """Pages that are none and pages of NaN and infinite scales among those of a wide tile's keys."""
+    rng = np.random.default_rng(hd)
+    n_q, n_kv, page, requests = 4, 2, 16, 130
+    lens, news = [320] + [2] * requests, [0] + [1] * requests
+    parent = [-1] + [0] * requests
+    shared_lens = [0] + [320 if i % 3 == 0 else 160 if i % 3 == 1 else 48 for i in range(requests)]
+    table, cache = _pool(rng, lens, page, n_kv, hd)
+    table[0, 2], table[0, 7] = -1, cache["ks"].shape[0] + 3
+    cache["vs"][table[0, 12], 0], cache["vs"][table[0, 13], 1], cache["ks"][table[0, 14], 1] = np.inf, np.nan, np.nan
+    starts, p = _planned(parent, shared_lens, lens, news, requests)
+    q = _f16(rng, requests, n_q, hd)
+    out = attend(Cache(cache), _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 1, 2, 1, 1 << 20)
+    got = host(out).astype(np.float64).reshape(requests, n_q, hd)
+    clean = dict(cache, ks=np.nan_to_num(cache["ks"], nan=0.01), vs=np.nan_to_num(cache["vs"], nan=0.01, posinf=0.01))
+    want, bound = px.attention(clean, q, starts, lens, table, parent, shared_lens, n_kv)
+    for i in range(requests):
+        if shared_lens[i + 1] == 320:   # sees the infinite V scale of head 0 and the NaNs of head 1
+            assert not np.isfinite(got[i, :2]).all() and np.isnan(got[i, 2:]).all(), i
+        else:
+            assert (np.abs(got[i] - want[i]) <= bound[i] + 2.0 ** -25).all(), i
+    release()
+
+
 def test_attention_prefix_small_bounds():
     """max_len and max_shared below the true lengths only shape the launch."""
     rng = np.random.default_rng(5)
