@@ -583,13 +583,13 @@ __device__ __forceinline__ void q_block(const QkvArgs& a, unsigned block) {
 template <int HD, int NCH>
 __global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void qkv_append_kernel(QkvArgs a) {
     __shared__ uint32_t red[2][4];
-    const unsigned b = blockIdx.x;
-    if (b >= a.kv_blocks) {
-        q_block<HD>(a, b - a.kv_blocks);
+    const unsigned at = blockIdx.x;
+    if (at >= a.kv_blocks) {
+        q_block<HD>(a, at - a.kv_blocks);
         return;
     }
-    const unsigned rest = b / a.windows;
-    append_block<HD, NCH, true>(a.kv, b % a.windows, rest % a.head_groups, rest / a.head_groups, red);
+    const unsigned rest = at / a.windows;
+    append_block<HD, NCH, true>(a.kv, at % a.windows, rest % a.head_groups, rest / a.head_groups, red);
 }
 
 // ------------------------------------------------------------------ the read

@@ -6,31 +6,50 @@
 // share any are listed parent by parent, in the order of rows within one: the
 // requests' numbers (parent, request) are sorted, and a prefix sum of their row
 // counts in that order is where each request's rows begin in the list.  Every
-// workgroup sorts for itself, in LDS, then fills its own share of the rows.
+// workgroup sorts for itself, then fills its own share of the rows.
+// The sort is bitonic; a wavefront holds 64 E consecutive numbers in registers, so that all
+// but the few exchanges between wavefronts go without LDS and barriers.
+#include <type_traits>
+
 #include "kv_pages.h"
 
 namespace bx {
 namespace {
 
 constexpr int kPrefixThreads = 512;
-constexpr int kPrefixRows = 1024;   // rows a workgroup
+constexpr int kPrefixRows = 512;   // rows a workgroup
 
 struct PrefixArgs {
     const int32_t *parent, *shared_lens, *starts, *lens, *pos_in;
-    int n_req, max_rows, slots;     // slots: a power of two, n_req or more
+    int n_req, max_rows, slots;     // slots: a power of two, n_req or more, at most 512 E
     int32_t *pos, *shared, *order, *groups, *group_starts;
 };
 
+// The value of lane l ^ J: without a trip through the LDS but for 4.
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (J == 1) return dpp_of<0xB1>(v);
+    else if constexpr (J == 2) return dpp_of<0x4E>(v);
+    else if constexpr (J == 8) return dpp_of<0x128>(v);   // the row of 16, half way round
+    else if constexpr (J == 16) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (uint32_t)((lane & 16) ? s[0] : s[1]);
+    } else if constexpr (J == 32) {
+        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (uint32_t)((lane & 32) ? s[0] : s[1]);
+    } else return (uint32_t)__shfl_xor((int)v, J);
+}
+
+template <int E>
 __global__ __launch_bounds__(kPrefixThreads) void prefix_plan_kernel(PrefixArgs a) {
     // the sorted numbers (parent << 12 | request; none: all ones), later the requests' shared keys
-    __shared__ uint32_t s_key[kPlanMaxReq];
-    __shared__ int32_t s_start[kPlanMaxReq + 1], s_at[kPlanMaxReq];
+    constexpr int N = kPrefixThreads * E;
+    static_assert(N <= kPlanMaxReq);
+    __shared__ uint32_t s_key[N];
+    __shared__ int32_t s_start[N + 1], s_at[N];
     __shared__ uint32_t red[2][kPrefixThreads / 64];
     const int t = threadIdx.x, n = a.n_req, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    auto shares = [&](int r) {
-        const int p = a.parent[r];
-        return p >= 0 && p < n && p != r ? max(0, min(a.shared_lens[r], a.lens[p])) : 0;
-    };
     // rows of request r; starts that do not ascend within the step's rows give none
     auto count = [&](int r) {
         const int b = s_start[r], e = s_start[r + 1];
@@ -38,23 +57,61 @@ __global__ __launch_bounds__(kPrefixThreads) void prefix_plan_kernel(PrefixArgs 
     };
     for (int r = t; r <= n; r += kPrefixThreads) s_start[r] = a.starts[r];
     __syncthreads();
-    for (int r = t; r < a.slots; r += kPrefixThreads)
-        s_key[r] = r < n && count(r) > 0 && shares(r) > 0 ? (uint32_t)a.parent[r] << 12 | (uint32_t)r : 0xffffffffu;
-    __syncthreads();
+    // number e of this thread: request 64 E wave + 64 i + lane
+    uint32_t key[E];
+    int share[E];
+    auto number = [&](int i) { return 64 * (E * wave + i) + lane; };
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int r = number(i), p = r < n ? a.parent[r] : -1;
+        share[i] = p >= 0 && p < n && p != r ? max(0, min(a.shared_lens[r], a.lens[p])) : 0;
+        key[i] = share[i] > 0 && count(r) > 0 ? (uint32_t)p << 12 | (uint32_t)r : 0xffffffffu;
+    }
 
     // ---- bitonic sort, ascending
-    for (int k = 2; k <= a.slots; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = t; i < a.slots / 2; i += kPrefixThreads) {
-                const int lo = (i & ~(j - 1)) * 2 + (i & (j - 1)), hi = lo + j;
-                const uint32_t x = s_key[lo], y = s_key[hi];
-                if ((x > y) == ((lo & k) == 0)) {
-                    s_key[lo] = y;
-                    s_key[hi] = x;
-                }
+    for (int k = 2; k <= a.slots; k <<= 1) {
+        uint32_t other[E];
+        auto keep = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int e = number(i);
+                key[i] = ((e & k) == 0) == ((e & j) == 0) ? min(key[i], other[i]) : max(key[i], other[i]);
             }
-            __syncthreads();
+        };
+        for (int j = k >> 1; j >= 64; j >>= 1) {
+            if (j >= 64 * E) {
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < E; ++i) s_key[number(i)] = key[i];
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < E; ++i) other[i] = s_key[number(i) ^ j];
+            } else {
+#pragma unroll
+                for (int d = 1; d < E; d *= 2)
+                    if (j == 64 * d)
+#pragma unroll
+                        for (int i = 0; i < E; ++i) other[i] = key[i ^ d];
+            }
+            keep(j);
         }
+        auto lanes = [&]<int J>(std::integral_constant<int, J>) {
+            if (J >= k) return;
+#pragma unroll
+            for (int i = 0; i < E; ++i) other[i] = lane_xor<J>(key[i]);
+            keep(J);
+        };
+        lanes(std::integral_constant<int, 32>{});
+        lanes(std::integral_constant<int, 16>{});
+        lanes(std::integral_constant<int, 8>{});
+        lanes(std::integral_constant<int, 4>{});
+        lanes(std::integral_constant<int, 2>{});
+        lanes(std::integral_constant<int, 1>{});
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; ++i) s_key[number(i)] = key[i];
+    __syncthreads();
 
     // ---- rows and groups before each of them, `per` consecutive ones a thread
     const int per = (a.slots + kPrefixThreads - 1) / kPrefixThreads, i0 = min(a.slots, t * per), i1 = min(a.slots, i0 + per);
@@ -105,7 +162,9 @@ __global__ __launch_bounds__(kPrefixThreads) void prefix_plan_kernel(PrefixArgs 
             a.group_starts[i] = (int)total[0];
         }
     __syncthreads();
-    for (int r = t; r < n; r += kPrefixThreads) s_key[r] = (uint32_t)shares(r);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (number(i) < n) s_key[number(i)] = (uint32_t)share[i];
     __syncthreads();
 
     // ---- the rows
@@ -159,7 +218,10 @@ int bx_prefix_plan(const int32_t* parent, const int32_t* shared_lens, const int3
     while (a.slots < n_req) a.slots *= 2;
     a.pos = pos; a.shared = shared; a.order = order; a.groups = groups; a.group_starts = group_starts;
     const unsigned grid = ((unsigned)max_rows + kPrefixRows - 1) / kPrefixRows;
-    prefix_plan_kernel<<<grid, kPrefixThreads, 0, as_stream(stream)>>>(a);
+    hipStream_t st = as_stream(stream);
+    if (a.slots <= kPrefixThreads) prefix_plan_kernel<1><<<grid, kPrefixThreads, 0, st>>>(a);
+    else if (a.slots <= 2 * kPrefixThreads) prefix_plan_kernel<2><<<grid, kPrefixThreads, 0, st>>>(a);
+    else prefix_plan_kernel<8><<<grid, kPrefixThreads, 0, st>>>(a);
     return launch_check("prefix_plan");
 }
 
