@@ -60,6 +60,8 @@ constexpr int kQaNarrowCols = 64;    // columns a request up to which narrow til
 constexpr int64_t kQaNarrowWork = (int64_t)1 << 27;   // bytes of K that they read, for more columns
 constexpr int kQsMaxSplits = 63;   // of shared keys; with the own ones a lane each in the join
 constexpr int kQsLeast = 4;        // tiles of 64 shared keys a part
+constexpr int kQcRows = 256, kQcGroups = 64;          // of a call whose tiles walk shared and own keys
+constexpr int64_t kQcBytes = (int64_t)60 << 20;       // of shared keys that these read (heads of 256: twice as many)
 constexpr int64_t kQsWideWork = (int64_t)1 << 25;   // pairs of a row's head and a shared key from which wide tiles pay
 constexpr int kQaWords = 32768;   // arrival counters of either kind of tile
 
@@ -93,6 +95,9 @@ struct QsArgs : QaArgs {
     float *part, *part_ml;
     int32_t* part_n;
 };
+
+// The same for few rows, where each request's tiles walk the shared keys and then its own.
+struct QcArgs : QsArgs {};
 
 // The first key that the row at position p sees (p below 0 where there are more rows than
 // keys; the window may be anything up to 2^31 - 1).
@@ -330,7 +335,7 @@ struct QaTile {
 template <int HD, bool NT, class A>
 __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block, unsigned char* smem) {
     constexpr int NC = HD / 64, NJ = HD / 16;
-    constexpr bool PART = std::is_same_v<A, QsArgs>;
+    constexpr bool PART = std::is_same_v<A, QsArgs>, CHAIN = std::is_same_v<A, QcArgs>;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
 
@@ -377,7 +382,38 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
     auto low = [&](int p) { return first_key(p, a.window); };
     const int plast = real ? p0 + tok : -1, plow = low(p0 + tok);
     const int kend = max(0, p0 + t_last + 1), k64 = low(p0 + t_first) / 64;
-    const int n64 = max(0, (kend + 63) / 64 - k64);
+    const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
+    const int last_block = max(0, (kend - 1) >> a.pshift);
+    // CHAIN: the first `before` keys of another request come first, n_pre tiles from its tile pre64
+    // on; a row at p sees those from far(p) on
+    int before = 0, pre64 = 0, n_pre = 0, pre_block = 0, base = 0;
+    const int32_t* pre_row = trow;
+    auto far = [&](int p) { return first_key((int)min((int64_t)base + p, (int64_t)0x7fffffff), a.window); };
+    if constexpr (CHAIN) {
+        base = a.shared[row0];
+        if (base > 0) {
+            // the group of the place that row0 has in the order, both found by all lanes at once
+            int at = -1;
+#pragma unroll
+            for (int n = 0; n < kQcRows / 64; ++n) {
+                const int i = 64 * n + lane;
+                const uint64_t hit = __ballot(i < a.rows && a.order[min(i, a.rows - 1)] == row0);
+                if (hit) at = 64 * n + __builtin_ctzll(hit);
+            }
+            const int k = min(lane, a.max_groups - 1), first = a.group_starts[k], of = a.groups[k];
+            const uint64_t upto = __ballot(lane < a.max_groups && first <= at);
+            const int rp = at >= 0 && upto ? __builtin_amdgcn_readlane(of, 63 - __builtin_clzll(upto)) : -1;
+            if (rp >= 0 && rp < a.n_req) {
+                before = (int)min((int64_t)min(base, max(0, a.lens[rp])), (int64_t)a.max_blocks << a.pshift);
+                pre64 = min(far(p0 + t_first), before) / 64;
+                n_pre = (before + 63) / 64 - pre64;
+                pre_block = max(0, (before - 1) >> a.pshift);
+                pre_row = a.table + (int64_t)rp * a.max_blocks;
+            }
+        }
+    }
+    const int n64 = n_pre + max(0, (kend + 63) / 64 - k64);
+    auto first_of = [&](int i) { return CHAIN && i < n_pre ? (pre64 + i) * 64 : (k64 + i - n_pre) * 64; };   // key of tile i
     // Tiles to a workgroup: the S-th part at least.  A round of its four wavefronts takes 1.8 us
     // and a record 0.33 us to join (heads of 128; the rounds of 256 twice that), so where that
     // leaves few, the square root of all (one request of 8,000 keys 18.6 -> 14.9 us, 16,000 20.7
@@ -389,10 +425,10 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
     const int tb = s * ku, te = min(n64, tb + ku);
 
     // ---- tiles: page ids two steps ahead, keys and values one
-    const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
-    const int last_block = max(0, (kend - 1) >> a.pshift);
     auto entry = [&](int i, int grp) {   // page of 16 keys of tile i
-        return *gptr<int32_t>(trow + min(((k64 + i) * 64 + 16 * grp) >> a.pshift, last_block));
+        const int b = (first_of(i) + 16 * grp) >> a.pshift;
+        if (CHAIN && i < n_pre) return *gptr<int32_t>(pre_row + min(b, pre_block));
+        return *gptr<int32_t>(trow + min(b, last_block));
     };
     auto load16 = [&]<class T>(const int8_t* p) {
         if constexpr (NT) return (T)__builtin_nontemporal_load(gptr<T>(p));
@@ -402,7 +438,7 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
     // every lane reads the pool's first bytes instead: the same loads in every turn of the
     // loop, so that a wait counts exactly those of its own tile, and no traffic.
     auto fetch = [&](QaTile<HD>& x, int i, int pk, int pv) {
-        const int key = (k64 + i) * 64;
+        const int key = first_of(i);
         const bool live = i < te;
         x.ok = pv >= 0 && pv < a.n_pages;
         const int64_t hk = (int64_t)(pk >= 0 && pk < a.n_pages ? pk : 0) * a.n_kv + g;
@@ -445,7 +481,12 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
     };
 
     auto compute = [&](const QaTile<HD>& x, int i) {
-        const int key = (k64 + i) * 64, kk = key + 16 * lg;
+        const int key = first_of(i), kk = key + 16 * lg;
+        // the last and first keys of the tile's first and last row, and of this lane's column
+        const bool pre = CHAIN && i < n_pre;
+        const int end0 = pre ? before - 1 : p0 + t_first, end1 = pre ? before - 1 : p0 + t_last;
+        const int low0 = pre ? far(p0 + t_first) : low(p0 + t_first), low1 = pre ? far(p0 + t_last) : low(p0 + t_last);
+        const int end = pre && real ? before - 1 : plast, from = pre ? far(p0 + tok) : plow;
         // S: lane l, element e of y[t] holds key 16 (l / 16) + 4 t + e of column l % 16
         float y[1][4][4];
 #pragma unroll
@@ -462,12 +503,12 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
             for (int e = 0; e < 4; ++e) y[0][t][e] = __builtin_fmaf((float)(h[e] * 256 + m[e]), 256.f, (float)w[e]);
             if (t == 1) __builtin_amdgcn_sched_barrier(0);   // two fragments' integer sums at a time
         }
-        const bool whole = key + 63 <= p0 + t_first && key >= low(p0 + t_last) && __all(x.ok);
-        sc.next(x.sv, x.ok && kk <= p0 + t_last && kk + 15 >= low(p0 + t_first));
+        const bool whole = key + 63 <= end0 && key >= low1 && __all(x.ok);
+        sc.next(x.sv, x.ok && kk <= end1 && kk + 15 >= low0);
         qa_h8 pb[1][4];
         qa_softmax<1, true>(
             y, x.sk, cfs, !whole,
-            [&](int, int t, int e) { return !x.ok || kk + 4 * t + e > plast || kk + 4 * t + e < plow; }, sc, mm, ll, pb,
+            [&](int, int t, int e) { return !x.ok || kk + 4 * t + e > end || kk + 4 * t + e < from; }, sc, mm, ll, pb,
             [&](const float (&al)[1]) { rescale(al[0]); });
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
@@ -729,7 +770,7 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned 
                 real[f] = false;
                 row[f] = 0;
             }
-            plast[f] = real[f] ? min(a.shared[row[f]], len) - 1 : -1;
+            plast[f] = real[f] ? max(0, min(a.shared[row[f]], len)) - 1 : -1;
             plow[f] = low(a.pos[row[f]]);
         } else {
             row[f] = row0 + tok;
@@ -1042,6 +1083,12 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qa_kernel(QaArgs
     qa_tile<HD, NT>(a, threadIdx.x, blockIdx.x, smem);
 }
 
+template <int HD>
+__global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qc_kernel(QcArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    qa_tile<HD, false>(a, threadIdx.x, blockIdx.x, smem);
+}
+
 // Both kinds of tiles in one launch, the long ones first: decode rows fill the CUs that
 // the chunks leave, or leave last.
 template <int HD>
@@ -1108,7 +1155,7 @@ __device__ __forceinline__ void qs_tile(const QsArgs& a, int r, int g, int s, in
         real = false;
         row = 0;
     }
-    const int plast = real ? min(a.shared[row], len) - 1 : -1, plow = first_key(a.pos[row], a.window);
+    const int plast = real ? max(0, min(a.shared[row], len)) - 1 : -1, plow = first_key(a.pos[row], a.window);
     qa_h8 qf[ND];
     {
         const uint16_t* const q = a.q + (int64_t)row * a.q_stride + (int64_t)head * HD + 8 * lh;
@@ -1638,7 +1685,7 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
 // columns at most, the keys of each over S workgroups.
 struct QsPlan {
     QaPlan own;
-    bool wide;
+    bool chain, wide;
     int groups, S;
     int64_t tiles;
     size_t part_bytes, ml_bytes, n_bytes;
@@ -1650,6 +1697,20 @@ QsPlan qs_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     p.own = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, max_len);
     p.groups = std::min({max_groups, n_req, rows});
     const int64_t G = n_q / n_kv, cus = num_cus();
+    // Few rows: every request's tiles of 16 columns walk the shared keys too, in one launch and
+    // without parts to join.  16 / 8 heads of 128, that against tiles of 128 columns, single tokens: 4 on 700
+    // keys 11.9 us and 15.8, on 8,000 (64 MB) 20.4 and 22.9, on 20,000 32.5 and 28.4; 16 on 700
+    // 12.9 and 16.2, on 2,000 (64 MB) 20.4 and 19.4, on 6,000 29.8 and 23.7; 40 on 700 (56 MB) 18.5
+    // and 19.3; 16 / 4 heads of 256, 32 rows of 4 requests on 4,000 (64 MB) 26.7 and 36.7.
+    const int64_t walks = std::max<int64_t>(std::min(n_req, rows), ((int64_t)rows * G + 15) / 16);
+    if (rows <= kQcRows && p.groups <= kQcGroups && walks * max_shared * n_kv * hd * 2 <= kQcBytes * (hd > 128 ? 2 : 1)) {
+        const QaPlan all = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, (int)std::min<int64_t>((int64_t)max_len + max_shared, 0x7fffffff));
+        if (!all.rows_too) {
+            p.own = all;
+            p.chain = true;
+            return p;
+        }
+    }
     // Tiles of 256 columns do more products for every operand from LDS and code converted, those of 128
     // leave more workgroups and share the chip better with the own keys.  32 / 8 heads of 128,
     // wide against 128: 1,640 rows (8 chunks and 32 single tokens) on prefixes of 9,000 and 6,750 keys
@@ -1820,8 +1881,15 @@ int bx_attention_prefix_q8_f16(const uint16_t* q, int64_t q_stride, int rows, co
     as.S = p.S;
     hipStream_t st = as_stream(stream);
     auto run = [&](auto hdc) -> int {
-        constexpr int HD = decltype(hdc)::value, lds = std::max(HD / 16 * 4096 + 512, 2 * QrShape<HD>::kBuf);
-        static std::atomic<uint64_t> allowed[2];
+        constexpr int HD = decltype(hdc)::value, own = HD / 16 * 4096 + 512, lds = std::max(own, 2 * QrShape<HD>::kBuf);
+        static std::atomic<uint64_t> allowed[3];
+        if (p.chain) {
+            if constexpr (own > 64 * 1024)
+                if (int rc = allow_lds(allowed[2], reinterpret_cast<const void*>(&qc_kernel<HD>), own, "attention_prefix_q8: LDS attribute"))
+                    return rc;
+            qc_kernel<HD><<<(unsigned)blocks, kQaThreads, own, st>>>(QcArgs{a});
+            return launch_check("attention_prefix_q8");
+        }
         if constexpr (HD <= 128) {
             if (p.wide) {
                 constexpr int wlds = QsWide<HD>::kLds;

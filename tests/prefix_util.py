@@ -77,9 +77,7 @@ def attention(cache, q, starts, lens, table, parent, shared_lens, n_kv, window=0
         key = np.arange(s + n)
         for i in range(m):
             at = s + int(lens[r]) - m + i
-            see = ok & (key <= at)
-            if int(lens[r]) - m + i < 0:
-                see &= key < s   # a row before the first own key still sees the shared ones
+            see = ok & ((key < s) | (key <= at))
             if window > 0:
                 see &= key > at - window
             if not see.any():

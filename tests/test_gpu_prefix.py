@@ -298,24 +298,30 @@ CASES = [  # lens, news, parent, shared_lens
                                             (4, 1, 256, 32)])
 @pytest.mark.parametrize("case", range(len(CASES)))
 @pytest.mark.parametrize("window", [0, 1, 37, 150])
-def test_attention_prefix(n_q, n_kv, hd, page, case, window):
+@pytest.mark.parametrize("path", ["walk", "tiles"])
+def test_attention_prefix(n_q, n_kv, hd, page, case, window, path):
+    """Tiles that walk the shared keys and then the own ones; tiles of shared keys that are joined with those of
+    the own ones (a bound on the shared keys that allows for far more)."""
     lens, news, parent, shared_lens = CASES[case]
     rng = np.random.default_rng(case * 7 + window + hd)
-    _case(rng, lens, news, parent, shared_lens, n_q, n_kv, hd, page, window)
+    loose = {} if path == "walk" else dict(max_shared=1 << 22)
+    _case(rng, lens, news, parent, shared_lens, n_q, n_kv, hd, page, window, **loose)
 
 
 @pytest.mark.parametrize("n_q,n_kv,hd,page,prefixes,requests,longest", [
     (8, 2, 128, 64, 1, 70, 1500), (4, 4, 64, 16, 9, 40, 700), (32, 8, 64, 32, 3, 45, 300), (3, 1, 256, 128, 2, 100, 600),
     (16, 1, 128, 16, 1, 33, 2000), (5, 5, 128, 32, 40, 41, 130)])
 @pytest.mark.parametrize("window", [0, 400])
-def test_attention_prefix_of_many_requests(n_q, n_kv, hd, page, prefixes, requests, longest, window):
+@pytest.mark.parametrize("path", ["walk", "tiles"])
+def test_attention_prefix_of_many_requests(n_q, n_kv, hd, page, prefixes, requests, longest, window, path):
     """Several tiles of 128 columns a group, groups of a few columns, keys over many workgroups."""
     rng = np.random.default_rng(requests + longest)
     lens = list(rng.integers(1, longest + 1, prefixes)) + list(rng.integers(1, 40, requests))
     news = [0] * prefixes + [1] * requests
     parent = [-1] * prefixes + list(rng.integers(-1, prefixes, requests))
     shared_lens = [0] * prefixes + [int(rng.integers(1, longest + 1)) for _ in range(requests)]
-    _case(rng, lens, news, parent, shared_lens, n_q, n_kv, hd, page, window, max_groups=prefixes + 1)
+    loose = {} if path == "walk" else dict(max_shared=1 << 18)
+    _case(rng, lens, news, parent, shared_lens, n_q, n_kv, hd, page, window, max_groups=prefixes + 1, **loose)
 
 
 @pytest.mark.parametrize("n_q,n_kv,hd,page", [(8, 2, 128, 64), (6, 2, 64, 16), (4, 1, 256, 32)])
@@ -395,14 +401,16 @@ def test_attention_prefix_of_nobody():
     table, cache = _pool(rng, lens, page, n_kv, hd)
     starts, p = _planned([-1] * 3, [0] * 3, lens, news, 7)
     q, c = _half(_f16(rng, 7, n_q, hd)), Cache(cache)
-    a = attend(c, q, dev(starts), _i32(lens), dev(table), p, n_q, 3, 300, 1, 1)
     b = c.attention(q, dev(starts), _i32(lens), dev(table), n_q, 3, 300)
-    np.testing.assert_array_equal(host(a).view(np.uint16), host(b).view(np.uint16))
+    for max_shared in (1, 1 << 22):
+        a = attend(c, q, dev(starts), _i32(lens), dev(table), p, n_q, 3, 300, 1, max_shared)
+        np.testing.assert_array_equal(host(a).view(np.uint16), host(b).view(np.uint16))
     release()
 
 
 @pytest.mark.parametrize("window", [0, 100])
-def test_attention_prefix_as_copies(window):
+@pytest.mark.parametrize("max_shared", [160, 1 << 22])
+def test_attention_prefix_as_copies(window, max_shared):
     """A prefix of whole pages that every request's table names by itself gives the same to the bound."""
     rng = np.random.default_rng(7)
     n_q, n_kv, hd, page = 8, 2, 128, 16
@@ -411,7 +419,7 @@ def test_attention_prefix_as_copies(window):
     table, cache = _pool(rng, lens, page, n_kv, hd)
     starts, p = _planned(parent, shared_lens, lens, news, 6)
     q, c = _f16(rng, 6, n_q, hd), Cache(cache)
-    a = host(attend(c, _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 4, 48, 1, 160, window)).astype(np.float64)
+    a = host(attend(c, _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 4, 48, 1, max_shared, window)).astype(np.float64)
     wide = np.full((4, 15), -1, np.int32)
     wide[:, :10] = table[0, :10]
     wide[1:, 10:10 + table.shape[1] - 1] = table[1:, :5][:, :wide.shape[1] - 10]
@@ -422,7 +430,8 @@ def test_attention_prefix_as_copies(window):
     release()
 
 
-def test_attention_prefix_pages_that_are_none():
+@pytest.mark.parametrize("max_shared", [100, 1 << 22])
+def test_attention_prefix_pages_that_are_none(max_shared):
     """Entries of the shared table that name no page hide their keys; all of them: the own keys alone."""
     rng = np.random.default_rng(8)
     n_q, n_kv, hd, page = 4, 2, 64, 16
@@ -432,13 +441,14 @@ def test_attention_prefix_pages_that_are_none():
     table[0, 1], table[0, 4], table[3, :] = -1, cache["ks"].shape[0], 2 ** 31 - 1
     starts, p = _planned(parent, shared_lens, lens, news, 3)
     q = _f16(rng, 3, n_q, hd)
-    out = attend(Cache(cache), _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 1, 30, 2, 100)
+    out = attend(Cache(cache), _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 1, 30, 2, max_shared)
     want, bound = px.attention(cache, q, starts, lens, table, parent, shared_lens, n_kv)
     assert (np.abs(host(out).astype(np.float64).reshape(want.shape) - want) <= bound + 2.0 ** -25).all()
     release()
 
 
-def test_attention_prefix_nan_stays_where_it_is_seen():
+@pytest.mark.parametrize("max_shared", [64, 1 << 22])
+def test_attention_prefix_nan_stays_where_it_is_seen(max_shared):
     """A page of NaN scale at the end of the prefix reaches only the rows that share it; one without
     own keys and without a seen shared one gives zeros."""
     rng = np.random.default_rng(9)
@@ -452,7 +462,7 @@ def test_attention_prefix_nan_stays_where_it_is_seen():
     q = _f16(rng, 4, n_q, hd)
     # window 1: the last row's only position is its own, whose key does not exist
     for window in (0, 1):
-        out = host(attend(Cache(cache), _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 1, 3, 1, 64, window))
+        out = host(attend(Cache(cache), _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 1, 3, 1, max_shared, window))
         out = out.astype(np.float64).reshape(4, n_q, hd)
         if window:
             assert np.isfinite(out).all()
@@ -465,7 +475,8 @@ def test_attention_prefix_nan_stays_where_it_is_seen():
     release()
 
 
-def test_attention_prefix_strided_rows_and_odd_addresses():
+@pytest.mark.parametrize("max_shared", [100, 1 << 22])
+def test_attention_prefix_strided_rows_and_odd_addresses(max_shared):
     rng = np.random.default_rng(10)
     t = torch()
     n_q, n_kv, hd, page, lens, news = 8, 2, 128, 16, [100, 33, 60], [0, 1, 20]
@@ -475,7 +486,7 @@ def test_attention_prefix_strided_rows_and_odd_addresses():
     w = n_q * hd
     wide = rng.standard_normal((21, w + 77)).astype(np.float16)
     out = t.full((21, w + 31), 9.0, dtype=t.float16, device="cuda")
-    attend(Cache(cache), _half(wide)[:, 3:3 + w], dev(starts), _i32(lens), dev(table), p, n_q, 20, 60, 1, 100, out=out[:, 5:5 + w])
+    attend(Cache(cache), _half(wide)[:, 3:3 + w], dev(starts), _i32(lens), dev(table), p, n_q, 20, 60, 1, max_shared, out=out[:, 5:5 + w])
     want, bound = px.attention(cache, wide[:, 3:3 + w].reshape(21, n_q, hd), starts, lens, table, parent, shared_lens, n_kv)
     got = host(out).astype(np.float64)
     assert (np.abs(got[:, 5:5 + w].reshape(21, n_q, hd) - want) <= bound + 2.0 ** -25).all()
@@ -528,9 +539,10 @@ def test_attention_prefix_pool_beyond_32_bits():
     far = np.where(table >= 0, ids[table], -1).astype(np.int32)
     starts, p = _planned([-1, 0], [0, 190], lens, [0, 1], 1)
     q = _f16(rng, 1, n_q, hd)
-    out = attend(c, _half(q), dev(starts), _i32(lens), dev(far), p, n_q, 1, 70, 1, 190)
     want, bound = px.attention(small, q, starts, lens, table, [-1, 0], [0, 190], n_kv)
-    assert (np.abs(host(out).astype(np.float64).reshape(want.shape) - want) <= bound + 2.0 ** -25).all()
+    for max_shared in (190, 1 << 22):
+        out = attend(c, _half(q), dev(starts), _i32(lens), dev(far), p, n_q, 1, 70, 1, max_shared)
+        assert (np.abs(host(out).astype(np.float64).reshape(want.shape) - want) <= bound + 2.0 ** -25).all()
     del c
     release()
     t.cuda.empty_cache()
@@ -539,8 +551,9 @@ def test_attention_prefix_pool_beyond_32_bits():
 # ------------------------------------------------- a step as a serving loop runs it
 
 @pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("max_shared", [None, 1 << 20])
 @pytest.mark.parametrize("n_q,n_kv,hd,page,news", [(4, 2, 64, 16, [0, 1, 1, 9]), (8, 2, 128, 64, [1]), (4, 1, 256, 32, [1, 30])])
-def test_serving_loop_with_prefixes(n_q, n_kv, hd, page, news, graph):
+def test_serving_loop_with_prefixes(n_q, n_kv, hd, page, news, graph, max_shared):
     """Plan, prefix plan, q / k / v and attention of a layer, step after step: two prefixes are written
     in chunks, requests join, fork elsewhere, end and start over; also captured once and replayed."""
     t = torch()
@@ -560,7 +573,8 @@ def test_serving_loop_with_prefixes(n_q, n_kv, hd, page, news, graph):
     out = t.empty_like(q_rot)
     delta, parent_d, shared_d = (t.zeros(n_req, dtype=t.int32, device="cuda") for _ in range(3))
     max_new, max_len = max(max(news), 40), width * page
-    nb = int(hip().bx_attention_prefix_q8_workspace_bytes(rows, n_req, n_q, n_kv, hd, max_new, max_len, 3, max_len))
+    max_shared = max_shared or max_len
+    nb = int(hip().bx_attention_prefix_q8_workspace_bytes(rows, n_req, n_q, n_kv, hd, max_new, max_len, 3, max_shared))
     ws = t.zeros(nb, dtype=t.uint8, device="cuda")
 
     def step():
@@ -568,7 +582,7 @@ def test_serving_loop_with_prefixes(n_q, n_kv, hd, page, news, graph):
         p.step(parent_d, shared_d, d.starts, d.past, d.pos)
         a, b = n_q * hd, (n_q + n_kv) * hd
         _qkv(c, x[:, :a], x[:, a:b], x[:, b:], gd, 1e-6, p.pos, cosd, sind, d.slots, n_q, q_out=q_rot)
-        attend(c, q_rot, d.starts, d.past, d.table, p, n_q, max_new, max_len, 3, max_len, out=out, ws=ws)
+        attend(c, q_rot, d.starts, d.past, d.table, p, n_q, max_new, max_len, 3, max_shared, out=out, ws=ws)
 
     captured = None
     for i in range(9):
