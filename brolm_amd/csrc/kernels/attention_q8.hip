@@ -28,6 +28,11 @@
 // A column tile's keys are split over workgroups where there are few tiles; each
 // leaves a record (O, m, l), the last one to arrive adds them in split order.
 //
+// Requests that share a prefix (bx_attention_prefix_q8_f16): its keys are walked once for
+// the rows of all of them, as columns of a tile of 128 (qa_rows_tile) or 256 (qs_tile), their own
+// keys as above in the same launch, and what either gave is joined.  A few rows walk the
+// shared keys by themselves (qc_kernel).  The rules stand at qs_plan.
+//
 // Single tokens are bound by their bytes: 48 requests of 8,000 to 16,000 keys, 8 KV heads of
 // 128, 212 us, 5.6 TB/s of codes (8 heads of 64: 107 us, 5.4; 4 of 256: 260 us, 4.4, one
 // wavefront a SIMD); one of 700 keys by latency (9.8 us: lengths, table, rows, the merge).
@@ -96,7 +101,9 @@ struct QsArgs : QaArgs {
     int32_t* part_n;
 };
 
-// The same for few rows, where each request's tiles walk the shared keys and then its own.
+// The same for few rows, where each request's tiles walk the shared keys and then its own: 4 rows on 700
+// shared keys and 90 own ones, 16 / 8 heads of 128, 11.0 us, the chain of loads of qa_kernel and
+// the group's.
 struct QcArgs : QsArgs {};
 
 // The first key that the row at position p sees (p below 0 where there are more rows than
@@ -1121,6 +1128,13 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qs_kernel(QsArgs
 // buffers and V three.
 // The rows of K are permuted in the operand so that a lane's 16 products of a fragment are keys 8
 // h .. + 7 and 16 + 8 h .. + 7 (h = lane / 32): P is an operand as it stands.
+// 1,640 rows, 32 / 8 heads of 128, on prefixes of 9,000 and 6,750 keys 286 us with their own keys, 790 TFLOP/s
+// (tiles of 128 columns, two workgroups a CU: 370); 114 rows on 30,000 118, 46.8 of it the products.  A tile takes 4,300
+// cycles, at the 1.5 to 1.6 GHz that the load leaves: twice 1,800 of 32 products (1,024 of them the
+// matrix unit's) with a conversion among them, beside 1,900 of softmax, which the other's products
+// slow by 1.4; without priority for the products it takes 4,780 (the 1,640 rows 312
+// us for 305).  One wavefront a SIMD with 64 columns, softmax and products of two tiles in one
+// order, moved its sums between the two halves of the register file: 114 rows 200 us for 122.
 template <int HD>
 struct QsShape {
     static constexpr int kTile = 64 * HD * 2;          // bytes of a K or V tile
@@ -1554,7 +1568,9 @@ __global__ __launch_bounds__(2 * kQaThreads, 2) void qs_wide_kernel(QsArgs share
 }
 
 // Joins what the own keys and the parts of the shared ones gave, a wavefront to a row and
-// head, in the order of the parts.
+// head, in the order of the parts.  57 rows of 32 heads of 128 on 6,000 keys 6.2 us, a launch and two
+// round trips.  Without it, the own tiles joining in a launch behind the shared ones, the two
+// kinds of work do not overlap: 54 us in all for 43.
 template <int HD>
 __global__ __launch_bounds__(kQaThreads) void qs_join_kernel(QsArgs a) {
     constexpr int LR = HD / 4, R = 64 / LR, B = 4;   // lanes a part, parts at once, loads on their way

@@ -541,8 +541,15 @@ __global__ __launch_bounds__(256, HD > 128 ? 3 : 4) void kv_append_kernel(Append
 //
 // Blocks below kv_blocks are the append's, with the head norm and the rotation of K in
 // registers between the load and the maximum; the others take the rows of q.  A wavefront
-// holds 512 / HD heads of a row at a time, eight elements a lane, `turns` times with the same
-// angles.
+// holds 512 / HD heads of a row at a time, eight elements a lane, kTurns times with the same
+// angles (7,389 rows of 32 heads: 63 us with the read behind it for one turn, 56 for two or four).
+// 16 rows, 16 / 8 heads of 128: 4.9 us, the append's chain of loads and the angles.  Prompts of
+// 7,389 rows, 32 / 8 heads of 128: 41.6 us for 167 MB, 4.0 TB/s (a copy has 5.2); the append is the
+// slower part, its runs as above (8 / 8 heads 25 us, 128 / 8 heads 111).  q's blocks first: 2
+// us more; streaming loads of q: as they are.  Heads of 256 spill 30 to 70 registers in the append
+// (7,389 rows of 16 / 4 heads 52 us).
+constexpr int kTurns = 2;
+
 struct QkvArgs {
     AppendArgs kv;
     unsigned windows, head_groups, kv_blocks;
@@ -550,30 +557,29 @@ struct QkvArgs {
     uint16_t* out;
     int64_t q_stride, out_stride;
     const uint16_t* q_gain;
-    int n_q, turns, parts;   // parts: wavefronts a row
+    int n_q, parts;   // parts: wavefronts a row
 };
 
 template <int HD>
 __device__ __forceinline__ void q_block(const QkvArgs& a, unsigned block) {
-    constexpr int HW = 512 / HD, MAXT = 4;
+    constexpr int HW = 512 / HD;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t item = (int64_t)block * 4 + wave, row = item / a.parts;
     if (row >= a.kv.rows) return;
-    const int head0 = (int)(item % a.parts) * HW * a.turns + lane / (HD / 8), d = 8 * (lane % (HD / 8));
+    const int head0 = (int)(item % a.parts) * HW * kTurns + lane / (HD / 8), d = 8 * (lane % (HD / 8));
     const int ps = a.kv.pos[row];
     if (ps < 0 || ps >= a.kv.tab_rows) return;
     const uint16_t* const x = a.q + row * a.q_stride + d;
-    u4v w[MAXT];
+    u4v w[kTurns];
     // heads behind the last one read it again and are not stored
 #pragma unroll
-    for (int i = 0; i < MAXT; ++i)
-        if (i < a.turns) w[i] = *reinterpret_cast<const any16*>(x + (int64_t)min(head0 + i * HW, a.n_q - 1) * HD);
+    for (int i = 0; i < kTurns; ++i)
+        w[i] = *reinterpret_cast<const any16*>(x + (int64_t)min(head0 + i * HW, a.n_q - 1) * HD);
     const u4v g = a.q_gain ? *reinterpret_cast<const any16*>(a.q_gain + d) : u4v{0u, 0u, 0u, 0u};
     const f4v c = *reinterpret_cast<const any_f4*>(a.kv.cos_t + (int64_t)ps * (HD / 2) + d / 2);
     const f4v s = *reinterpret_cast<const any_f4*>(a.kv.sin_t + (int64_t)ps * (HD / 2) + d / 2);
 #pragma unroll
-    for (int i = 0; i < MAXT; ++i) {
-        if (i >= a.turns) break;
+    for (int i = 0; i < kTurns; ++i) {
         const u4v y = norm_rope8<HD>(w[i], a.q_gain != nullptr, g, a.kv.eps, c, s);
         const int head = head0 + i * HW;
         if (head < a.n_q) *reinterpret_cast<any16*>(a.out + row * a.out_stride + (int64_t)head * HD + d) = y;
@@ -794,18 +800,17 @@ int bx_qkv_append_q8_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k,
     if (rows <= 0 || n_q <= 0 || tab_rows <= 0 || k_stride < width || v_stride < width || q_stride < q_width ||
         q_out_stride < q_width)
         return fail(BX_EINVAL, "qkv_append_q8: bad shape");
+    if (n_q > 1 << 24) return fail(BX_EUNSUPPORTED, "qkv_append_q8: too many rows and heads");
     if ((q_gain == nullptr) != (k_gain == nullptr)) return fail(BX_EINVAL, "qkv_append_q8: one of two gains");
     if (!(eps >= 0.f)) return fail(BX_EINVAL, "qkv_append_q8: bad eps");
     QkvArgs a{};
     a.kv = append_args(k, k_stride, v, v_stride, rows, n_kv, slots, page, n_pages, Kc, Vc, k_scale, v_scale);
     a.kv.gain = k_gain; a.kv.eps = eps; a.kv.pos = pos; a.kv.cos_t = cos_tab; a.kv.sin_t = sin_tab; a.kv.tab_rows = tab_rows;
-    const int per = heads_of(page), at_once = 512 / hd;
+    const int per = heads_of(page), at_once = 512 / hd * kTurns;
     a.windows = ((unsigned)rows + a.kv.window - 1) / a.kv.window;
     a.head_groups = (unsigned)((n_kv + per - 1) / per);
     a.q = q; a.q_stride = q_stride; a.out = q_out; a.out_stride = q_out_stride; a.q_gain = q_gain; a.n_q = n_q;
-    const int steps = (n_q + at_once - 1) / at_once;
-    a.turns = rows <= 256 ? 1 : std::min(4, steps);
-    a.parts = (steps + a.turns - 1) / a.turns;
+    a.parts = (n_q + at_once - 1) / at_once;
     const int64_t kv_blocks = (int64_t)a.windows * a.head_groups * 2, blocks = kv_blocks + ((int64_t)rows * a.parts + 3) / 4;
     if (blocks > 0x7fffffff) return fail(BX_EUNSUPPORTED, "qkv_append_q8: too many rows and heads");
     a.kv_blocks = (unsigned)kv_blocks;

@@ -9,6 +9,8 @@
 // workgroup sorts for itself, then fills its own share of the rows.
 // The sort is bitonic; a wavefront holds 64 E consecutive numbers in registers, so that all
 // but the few exchanges between wavefronts go without LDS and barriers.
+// Latency bounds it (loads in series, the sort's steps, the rows): 17 requests 4.0 us; 740 with
+// 25,000 rows 10.0 (17.9 with the numbers in LDS and a barrier a step); 4,040 requests 28.
 #include <type_traits>
 
 #include "kv_pages.h"

@@ -446,12 +446,14 @@ int bx_qkv_append_q8_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k,
 /* bx_attention_paged_q8_f16 for a step with shared prefixes: a row of request r
  * attends the first shared[row] keys of its group's request, then r's own keys up to
  * its own position; with a window, the last `window` of these.  Shared keys are read
- * once for 128 / (n_q / n_kv) rows of a group.  starts, lens, table and the cache as there
- * (own keys); pos, shared, order, groups and group_starts as bx_prefix_plan writes them.
- * max_new and max_len (own keys) as there; max_groups >= the number of groups (rows
- * of groups behind it may be left as they are); max_shared (about the most shared keys)
- * shapes the launch.  The weights of shared keys enter the product with V as those of long chunks
- * do; everything else as there.
+ * once for 128 or 256 / (n_q / n_kv) rows of a group; where rows are so few that this would
+ * not pay, once a request.  starts, lens, table and the cache as there (own keys); pos,
+ * shared, order, groups and group_starts as bx_prefix_plan writes them.
+ * max_new and max_len (own keys) as there, but a row of a request with more new rows is
+ * undefined; max_groups >= the number of groups (the rows of others are undefined); max_shared
+ * (about the most shared keys) shapes the launch.  Where shared keys are read once for many rows
+ * their scores take q as it is, and their weights enter the product with V to 2^-11, as those of
+ * long chunks; everything else as there.  One page of one layer (n_kv * page * hd) is below 2 GiB.
  * ws: bx_attention_prefix_q8_workspace_bytes(...) bytes with the same arguments (a
  * workspace for several shapes: the largest), 16-byte aligned, its first 512 KB zeroed
  * once before the first use; calls sharing one must not overlap. */

@@ -46,7 +46,8 @@ QKV = [("q", P), ("q_stride", 2048), ("k", P), ("k_stride", 1024), ("v", P), ("v
     (dict(eps=-1.0), EINVAL, "eps"), (dict(eps=float("nan")), EINVAL, "eps"), (dict(n_kv=0), EINVAL, "cache shape"),
     (dict(n_pages=0), EINVAL, "cache shape"), (dict(page=48), EUNSUPPORTED, "pages hold"), (dict(hd=96), EUNSUPPORTED, "head_dim"),
     (dict(vc=C.c_void_p(0x1008)), EINVAL, "aligned"),
-    (dict(rows=2 ** 31 - 1, n_kv=64, k_stride=8192, v_stride=8192), EUNSUPPORTED, "too many")])
+    (dict(rows=2 ** 31 - 1, n_kv=64, k_stride=8192, v_stride=8192), EUNSUPPORTED, "too many"),
+    (dict(n_q=(1 << 24) + 1, q_stride=1 << 32, q_out_stride=1 << 32), EUNSUPPORTED, "too many")])
 def test_qkv_append_refuses(native, kw, code, word):
     _refused(native, "bx_qkv_append_q8_f16", _with(QKV, **kw), code, word)
 
@@ -69,7 +70,8 @@ ATTN = [("q", P), ("q_stride", 2048), ("rows", 5), ("starts", P), ("lens", P), (
     (dict(out_stride=2047), EINVAL, "stride"), (dict(max_blocks=1 << 25), EUNSUPPORTED, "tokens a request"),
     (dict(ws_bytes=16), EINVAL, "workspace"), (dict(ws=C.c_void_p(0x1008)), EINVAL, "workspace"),
     (dict(hd=80), EUNSUPPORTED, "head_dim"), (dict(page=0), EUNSUPPORTED, "pages hold"),
-    (dict(kc=C.c_void_p(0x1001)), EINVAL, "aligned")])
+    (dict(kc=C.c_void_p(0x1001)), EINVAL, "aligned"),
+    (dict(n_q=1 << 18, n_kv=1 << 18, page=128, q_stride=1 << 26, out_stride=1 << 26), EUNSUPPORTED, "2^31 bytes")])
 def test_attention_prefix_refuses(native, kw, code, word):
     _refused(native, "bx_attention_prefix_q8_f16", _with(ATTN, **kw), code, word)
 
@@ -79,7 +81,8 @@ def test_attention_prefix_workspace_query(native):
     own = native.hip().bx_attention_paged_q8_workspace_bytes
     assert f(0, 1, 16, 8, 128, 1, 100, 1, 100) == 0 and f(1, 1, 15, 8, 128, 1, 100, 1, 100) == 0
     assert f(1, 1, 16, 8, 128, 1, 100, 0, 100) == 0 and f(1, 1, 16, 8, 128, 1, 100, 1, 0) == 0
-    assert f(4, 5, 16, 8, 128, 1, 100, 1, 100) > own(4, 5, 16, 8, 128, 1, 100)
+    assert f(4, 5, 16, 8, 128, 1, 100, 1, 100) >= own(4, 5, 16, 8, 128, 1, 100)
+    assert f(300, 5, 16, 8, 128, 60, 100, 1, 100) > own(300, 5, 16, 8, 128, 60, 100)
     assert f(4, 5, 16, 8, 128, 1, 100, 1, 100000) > f(4, 5, 16, 8, 128, 1, 100, 1, 100)
 
 
