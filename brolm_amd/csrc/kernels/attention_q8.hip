@@ -392,10 +392,10 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
     const int32_t* const trow = a.table + (int64_t)r * a.max_blocks;
     const int last_block = max(0, (kend - 1) >> a.pshift);
     // CHAIN: the first `before` keys of another request come first, n_pre tiles from its tile pre64
-    // on; a row at p sees those from far(p) on
+    // on; a row at p sees those from far(p) on (one before its first own key: all)
     int before = 0, pre64 = 0, n_pre = 0, pre_block = 0, base = 0;
     const int32_t* pre_row = trow;
-    auto far = [&](int p) { return first_key((int)min((int64_t)base + p, (int64_t)0x7fffffff), a.window); };
+    auto far = [&](int p) { return p < 0 ? 0 : first_key((int)min((int64_t)base + p, (int64_t)0x7fffffff), a.window); };
     if constexpr (CHAIN) {
         base = a.shared[row0];
         if (base > 0) {

@@ -445,9 +445,10 @@ int bx_qkv_append_q8_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k,
 
 /* bx_attention_paged_q8_f16 for a step with shared prefixes: a row of request r
  * attends the first shared[row] keys of its group's request, then r's own keys up to
- * its own position; with a window, the last `window` of these.  Shared keys are read
- * once for 128 or 256 / (n_q / n_kv) rows of a group; where rows are so few that this would
- * not pay, once a request.  starts, lens, table and the cache as there (own keys); pos,
+ * its own position; with a window, the last `window` of these (but all shared keys for a row
+ * before its request's first own key, more rows than keys).  Shared keys are read once for
+ * 128 or 256 / (n_q / n_kv) rows of a group; where rows are so few that this would not pay,
+ * once a request.  starts, lens, table and the cache as there (own keys); pos,
  * shared, order, groups and group_starts as bx_prefix_plan writes them.
  * max_new and max_len (own keys) as there, but a row of a request with more new rows is
  * undefined; max_groups >= the number of groups (the rows of others are undefined); max_shared

@@ -521,6 +521,60 @@ def test_attention_prefix_one_workspace_for_many_shapes_and_repeats():
     release()
 
 
+@pytest.mark.parametrize("max_shared", [100, 1 << 22])
+def test_attention_prefix_more_rows_than_keys(max_shared):
+    """Rows before the first own key attend all shared keys, the others the last `window` of theirs."""
+    rng = np.random.default_rng(17)
+    n_q, n_kv, hd, page, window = 8, 2, 128, 16, 37
+    lens, news, parent, shared_lens = [100, 2, 0], [0, 5, 2], [-1, 0, 0], [0, 100, 90]
+    table, cache = _pool(rng, lens, page, n_kv, hd)
+    starts, p = _planned(parent, shared_lens, lens, news, 7)
+    q = _f16(rng, 7, n_q, hd)
+    got = host(attend(Cache(cache), _half(q), dev(starts), _i32(lens), dev(table), p, n_q, 5, 100, 1, max_shared, window=window))
+    before = np.array([True, True, True, False, False, True, True])
+    whole, last = (px.attention(cache, q, starts, lens, table, parent, shared_lens, n_kv, w) for w in (0, window))
+    want, bound = (np.where(before[:, None, None], x, y) for x, y in zip(whole, last))
+    assert (np.abs(got.astype(np.float64).reshape(want.shape) - want) <= bound + 2.0 ** -25).all()
+    release()
+
+
+def test_attention_prefix_captured_calls_share_a_workspace():
+    """Graphs of calls of several kinds on one workspace, replayed in turn with eager calls between."""
+    t = torch()
+    rng = np.random.default_rng(19)
+    n_q, n_kv, hd, page = 8, 2, 128, 64
+    shapes = [([700, 300, 9], [0, 1, 1], [-1, 0, 0], [0, 700, 650]),                       # few rows
+              ([900] + [60] * 70, [0] + [4] * 70, [-1] + [0] * 70, [0] + [900] * 70),       # tiles of 128 columns
+              ([9000, 400, 300], [0, 400, 300], [-1, 0, 0], [0, 9000, 8000])]               # tiles of 256
+    calls, sizes = [], []
+    for lens, news, parent, shared_lens in shapes:
+        table, cache = _pool(rng, lens, page, n_kv, hd)
+        rows = sum(news)
+        starts, p = _planned(parent, shared_lens, lens, news, rows)
+        out = t.zeros((rows, n_q * hd), dtype=t.float16, device="cuda")
+        calls.append(((Cache(cache), _half(_f16(rng, rows, n_q, hd)), dev(starts), _i32(lens), dev(table), p, n_q, max(news),
+                       max(lens), 1, lens[0]), out))
+        sizes.append(int(hip().bx_attention_prefix_q8_workspace_bytes(rows, len(lens), n_q, n_kv, hd, max(news), max(lens), 1,
+                                                                      lens[0])))
+    ws = t.zeros(max(sizes), dtype=t.uint8, device="cuda")
+    alone, graphs = [], []
+    for args, out in calls:
+        alone.append(host(attend(*args, out=out, ws=ws)))
+        graphs.append(t.cuda.CUDAGraph())
+        with t.cuda.graph(graphs[-1]):
+            attend(*args, out=out, ws=ws)
+    for turn in range(6):
+        for i in rng.permutation(len(calls)):
+            calls[i][1].zero_()
+            graphs[i].replay()
+            k = int(rng.integers(len(calls)))
+            got = host(calls[i][1])
+            np.testing.assert_array_equal(got, alone[i], err_msg=f"turn {turn}, call {i}")
+            attend(*calls[k][0], out=calls[k][1], ws=ws)
+            np.testing.assert_array_equal(host(calls[k][1]), alone[k])
+    release()
+
+
 def test_attention_prefix_pool_beyond_32_bits():
     """Shared pages whose codes lie more than 2^32 bytes into the pool."""
     t = torch()
