@@ -66,7 +66,7 @@ constexpr int64_t kQaNarrowWork = (int64_t)1 << 27;   // bytes of K that they re
 constexpr int kQsMaxSplits = 63;   // of shared keys; with the own ones a lane each in the join
 constexpr int kQsLeast = 4;        // tiles of 64 shared keys a part
 constexpr int kQcRows = 256, kQcGroups = 64;          // of a call whose tiles walk shared and own keys
-constexpr int64_t kQcBytes = (int64_t)60 << 20;       // of shared keys that these read (heads of 256: twice as many)
+constexpr int64_t kQcBytes = (int64_t)60 << 20;       // of shared keys that these read (heads of 256: half as many more)
 constexpr int64_t kQsWideWork = (int64_t)1 << 25;   // pairs of a row's head and a shared key from which wide tiles pay
 constexpr int kQaWords = 32768;   // arrival counters of either kind of tile
 
@@ -680,13 +680,13 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
 // (one barrier a tile; 16-byte chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with
 // q as it is.
 // Prompts of 2,047 and 2,010 rows, 32 / 8 heads of 128: 101 us, 667 TFLOP/s (heads of 64: 72 us;
-// 16 / 4 heads of 256: 166); 1,500 rows at 12,000 keys 800.  What bounds it: two wavefronts a
+// 16 / 4 heads of 256: 127); 1,500 rows at 12,000 keys 800.  What bounds it: two wavefronts a
 // SIMD (245 registers, 64 KB of LDS a workgroup), whose VALU work (exponents, exponentials,
 // sums and the conversion of codes, about 360 instructions for every 64 matrix instructions)
 // fills 59 % of the time, the matrix cores a quarter, and 28 % of whose cycles wait, for
 // counters or at the tile's barrier.  Eight wavefronts that share a tile convert half as much
 // for 5 % and leave a batch half as many workgroups; holding the next tile's conversion over
-// the softmax spills (194 us).  Heads of 256 spill as it is (30 registers), at one wavefront a SIMD.
+// the softmax spills (194 us).  Heads of 256 leave one wavefront a SIMD.
 template <int HD>
 struct QrShape {
     static constexpr int CH = HD / 8;             // 16-byte chunks of a K row
@@ -719,7 +719,9 @@ template <int HD, bool SHARED, class A>
 __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned block, unsigned blocks,
                                              unsigned char* smem) {
     using S = QrShape<HD>;
-    constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI, KB = HD > 128 ? 1 : 2;
+    constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI;
+    // operands of K on their way from LDS, the steps that the compiler may order, and fragments of V
+    constexpr int KA = HD > 128 ? 4 : NS, KS = HD > 128 ? 1 : NS, VB = HD > 128 ? 3 : 2;
     constexpr bool PART = std::is_same_v<A, QsArgs>;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
@@ -894,6 +896,26 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned 
         for (int j = 0; j < NJ; ++j) o[f][j] = qa_f4{0.f, 0.f, 0.f, 0.f};
     }
     const float sl2 = 1.4426950408889634f / sqrtf((float)HD), cfs[2] = {sl2, sl2};
+    // Heads of 256: q and O in the half of the register file that only matrix instructions reach, but for
+    // the few tiles that move the maximum; left to itself the compiler moved most of them every tile and
+    // spilled (2,047 and 2,010 rows 159 -> 127 us with the reads ahead of their products below, 24 x 8 rows on 12,000
+    // shared keys 105 -> 87)
+    auto pin_q = [&] {
+        if constexpr (HD > 128) {
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int d = 0; d < NS; ++d) asm volatile("" : "+a"(qf[f][d]));
+        }
+    };
+    auto pin_o = [&] {
+        if constexpr (HD > 128) {
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) asm volatile("" : "+a"(o[f][j]));
+        }
+    };
     QaScale sc;
     if (tb < te) {
         look(tb);
@@ -914,31 +936,33 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned 
         scales();   // of the next tile
         look(i + 2);
         if (works && key <= last_max && key + 63 >= low_min) {
-            // fragments from LDS a step ahead of the products that take them (heads of 256
-            // have no registers for K's)
+            // operands from LDS ahead of the products that take them: a fragment's parts, heads of 256
+            // (whose registers hold no more) four of K, two head dims' of V
             float y[2][4][4];
-            qa_h8 kf[KB][NS];
-            auto k_read = [&](int t) {
-                const int kr = 16 * (lc >> 2) + 4 * t + (lc & 3);
-#pragma unroll
-                for (int d = 0; d < NS; ++d)
-                    kf[t % KB][d] = *reinterpret_cast<const qa_h8*>(kt + kr * HD * 2 + (((4 * d + lg) ^ S::kswz(kr)) << 4));
+            pin_q();
+            constexpr int N = 4 * NS;   // steps: part k % NS of fragment k / NS
+            qa_h8 kf[KA + 1];
+            auto k_read = [&](int k) {
+                const int kr = 16 * (lc >> 2) + 4 * (k / NS) + (lc & 3);
+                kf[k % (KA + 1)] = *reinterpret_cast<const qa_h8*>(kt + kr * HD * 2 + (((4 * (k % NS) + lg) ^ S::kswz(kr)) << 4));
             };
-            if (KB > 1) k_read(0);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (t + KB - 1 < 4) k_read(t + KB - 1);
-                if constexpr (KB > 1) __builtin_amdgcn_sched_barrier(0);
-                qa_f4 acc[2] = {qa_f4{0.f, 0.f, 0.f, 0.f}, qa_f4{0.f, 0.f, 0.f, 0.f}};
+            for (int k = 0; k < KA; ++k) k_read(k);
+            qa_f4 acc[2];
 #pragma unroll
-                for (int d = 0; d < NS; ++d)
+            for (int k = 0; k < N; ++k) {
+                if (k + KA < N) k_read(k + KA);
+                if (k % KS == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    if (k % NS == 0) acc[f] = qa_f4{0.f, 0.f, 0.f, 0.f};
+                    acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k % (KA + 1)], qf[f][k % NS], acc[f], 0, 0, 0);
+                }
+                if (k % NS == NS - 1)
 #pragma unroll
                     for (int f = 0; f < 2; ++f)
-                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t % KB][d], qf[f][d], acc[f], 0, 0, 0);
 #pragma unroll
-                for (int f = 0; f < 2; ++f)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[f][t][e] = acc[f][e];
+                        for (int e = 0; e < 4; ++e) y[f][k / NS][e] = acc[f][e];
             }
             const bool whole = key + 63 <= last_min && key >= low_max && __all(ok);
             const int kk = key + 16 * lg;
@@ -948,28 +972,31 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned 
                 y, sk, cfs, !whole,
                 [&](int f, int t, int e) { return !ok || kk + 4 * t + e > plast[f] || kk + 4 * t + e < plow[f]; }, sc, m, l, pb,
                 [&](const float (&al)[2]) {
+                    pin_o();
 #pragma unroll
                     for (int f = 0; f < 2; ++f)
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) o[f][j] *= al[f];
+                    pin_o();
                 });
-            qa_h8 vf[2][2];
+            qa_h8 vf[VB][2];
             auto v_read = [&](int j) {
                 const int d = 16 * j + lc;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
-                    vf[j % 2][u] = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ S::vswz(d)) << 4));
+                    vf[j % VB][u] = *reinterpret_cast<const qa_h8*>(vt + d * 128 + (((2 * lg + u) ^ S::vswz(d)) << 4));
             };
-            v_read(0);
+#pragma unroll
+            for (int j = 0; j < VB - 1; ++j) v_read(j);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                if (j + 1 < NJ) v_read(j + 1);
+                if (j + VB - 1 < NJ) v_read(j + VB - 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int f = 0; f < 2; ++f)
-                        o[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j % 2][u], pb[f][u], o[f][j], 0, 0, 0);
+                        o[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j % VB][u], pb[f][u], o[f][j], 0, 0, 0);
             }
         }
         if (i + 1 < te) {
@@ -1670,8 +1697,8 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         // would run alone at the end.  32 / 8 heads of 128: 400 rows beside 7 single tokens at
         // 6,000 keys 77 us in four parts, 97 in five (520 workgroups), 90 in three; 500 beside
         // 39 at 4,000 89 in three, 104 in four; three of 126 to 200 rows and one token at 3,000
-        // 53 in three, 64 in four (544).  16 / 4 heads of 256, 500 rows at 4,000 90 in four,
-        // 122 in eight.
+        // 53 in three, 64 in four (544).  16 / 4 heads of 256, 500 rows at 4,000 70 in four,
+        // 97 in eight.
         p.tiles = (int64_t)rows * G / 128 + n_req;
         const int64_t tb = p.tiles * n_kv, rec = (int64_t)hd * 512 + 1024, slots = hd > 128 ? cus : 2 * cus;
         const int64_t singles = hd > 128 ? 0 : std::min(cus / 2, (n_req - longer) * n_kv * p.S);
@@ -1682,7 +1709,7 @@ QaPlan qa_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
         // keys and about four tiles' time to begin and to join (32 / 8 heads of 128, 1,500 rows
         // at 8,000 keys: one round of 376 workgroups 281 us, 254 in parts; 1,100 beside 29
         // single tokens at 12,000 447 and 358; 16 / 4 heads of 256, three chunks of 326 to 400
-        // rows at 2,000: 148 workgroups 142, 444 127).
+        // rows at 2,000: 148 workgroups 101, 444 82).
         auto time = [&](int64_t n) { return ((likely * n + slots - 1) / slots) * (max_len / 64.0 / n + 4.0); };
         const double once = time(Sr);
         double least = 0.85 * once;
@@ -1717,9 +1744,10 @@ QsPlan qs_plan(int rows, int n_req, int n_q, int n_kv, int hd, int max_new, int 
     // without parts to join.  16 / 8 heads of 128, that against tiles of 128 columns, single tokens: 4 on 700
     // keys 11.9 us and 15.8, on 8,000 (64 MB) 20.4 and 22.9, on 20,000 32.5 and 28.4; 16 on 700
     // 12.9 and 16.2, on 2,000 (64 MB) 20.4 and 19.4, on 6,000 29.8 and 23.7; 40 on 700 (56 MB) 18.5
-    // and 19.3; 16 / 4 heads of 256, 32 rows of 4 requests on 4,000 (64 MB) 26.7 and 36.7.
+    // and 19.3; 16 / 4 heads of 256, 32 rows of 4 requests on 4,000 (64 MB) 26.4 and 32.6, 64 of 8 (131 MB)
+    // 38.2 and 34.1, 8 single tokens 24.2 and 27.0, 16 (131 MB) 36.6 and 31.5.
     const int64_t walks = std::max<int64_t>(std::min(n_req, rows), ((int64_t)rows * G + 15) / 16);
-    if (rows <= kQcRows && p.groups <= kQcGroups && walks * max_shared * n_kv * hd * 2 <= kQcBytes * (hd > 128 ? 2 : 1)) {
+    if (rows <= kQcRows && p.groups <= kQcGroups && walks * max_shared * n_kv * hd * 2 <= kQcBytes * (hd > 128 ? 3 : 2) / 2) {
         const QaPlan all = qa_plan(rows, n_req, n_q, n_kv, hd, max_new, (int)std::min<int64_t>((int64_t)max_len + max_shared, 0x7fffffff));
         if (!all.rows_too) {
             p.own = all;
