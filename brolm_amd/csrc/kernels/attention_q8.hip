@@ -679,7 +679,7 @@ __device__ __forceinline__ void qa_tile(const A& a, unsigned tid, unsigned block
 // two tiles ahead, converts them once for the 128 columns and stores them double-buffered
 // (one barrier a tile; 16-byte chunks XOR-swizzled).  S^T = K Q^T is then one FP16 product with
 // q as it is.
-// Prompts of 2,047 and 2,010 rows, 32 / 8 heads of 128: 101 us, 667 TFLOP/s (heads of 64: 72 us;
+// Prompts of 2,047 and 2,010 rows, 32 / 8 heads of 128: 101 us, 667 TFLOP/s (heads of 64: 68 us;
 // 16 / 4 heads of 256: 127); 1,500 rows at 12,000 keys 800.  What bounds it: two wavefronts a
 // SIMD (245 registers, 64 KB of LDS a workgroup), whose VALU work (exponents, exponentials,
 // sums and the conversion of codes, about 360 instructions for every 64 matrix instructions)
@@ -720,8 +720,8 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned 
                                              unsigned char* smem) {
     using S = QrShape<HD>;
     constexpr int NS = HD / 32, NJ = HD / 16, NI = S::NI;
-    // operands of K on their way from LDS, the steps that the compiler may order, and fragments of V
-    constexpr int KA = HD > 128 ? 4 : NS, KS = HD > 128 ? 1 : NS, VB = HD > 128 ? 3 : 2;
+    // operands of K on their way from LDS, and fragments of V
+    constexpr int KA = HD > 128 ? 4 : NS, VB = HD > 128 ? 3 : 2;
     constexpr bool PART = std::is_same_v<A, QsArgs>;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lc = lane & 15, lg = lane >> 4, G = a.G, page = 1 << a.pshift;
@@ -952,7 +952,7 @@ __device__ __forceinline__ void qa_rows_tile(const A& a, unsigned tid, unsigned 
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 if (k + KA < N) k_read(k + KA);
-                if (k % KS == 0) __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int f = 0; f < 2; ++f) {
                     if (k % NS == 0) acc[f] = qa_f4{0.f, 0.f, 0.f, 0.f};
