@@ -101,9 +101,8 @@ struct QsArgs : QaArgs {
     int32_t* part_n;
 };
 
-// The same for few rows, where each request's tiles walk the shared keys and then its own: 4 rows on 700
-// shared keys and 90 own ones, 16 / 8 heads of 128, 11.0 us, the chain of loads of qa_kernel and
-// the group's.
+// The same for few rows, where each request's tiles walk the shared keys and then its own: 4 rows on
+// 700 shared keys, 16 / 8 heads of 128, 11 us, the chain of loads of qa_kernel and the group's.
 struct QcArgs : QsArgs {};
 
 // The first key that the row at position p sees (p below 0 where there are more rows than
@@ -1155,12 +1154,12 @@ __global__ __launch_bounds__(kQaThreads, HD > 128 ? 1 : 2) void qs_kernel(QsArgs
 // buffers and V three.
 // The rows of K are permuted in the operand so that a lane's 16 products of a fragment are keys 8
 // h .. + 7 and 16 + 8 h .. + 7 (h = lane / 32): P is an operand as it stands.
-// 1,640 rows, 32 / 8 heads of 128, on prefixes of 9,000 and 6,750 keys 286 us with their own keys, 790 TFLOP/s
-// (tiles of 128 columns, two workgroups a CU: 370); 114 rows on 30,000 118, 46.8 of it the products.  A tile takes 4,300
-// cycles, at the 1.5 to 1.6 GHz that the load leaves: twice 1,800 of 32 products (1,024 of them the
-// matrix unit's) with a conversion among them, beside 1,900 of softmax, which the other's products
-// slow by 1.4; without priority for the products it takes 4,780 (the 1,640 rows 312
-// us for 305).  One wavefront a SIMD with 64 columns, softmax and products of two tiles in one
+// 1,640 rows, 32 / 8 heads of 128, on prefixes of 9,000 and 6,750 keys 286 us with their own keys,
+// 790 TFLOP/s (tiles of 128 columns, two workgroups a CU: 370); 114 rows on 30,000 118, 46.8 of it
+// the products.  A tile takes 4,300 cycles, at the 1.5 to 1.6 GHz that the load leaves: twice 1,800
+// of 32 products (1,024 of them the matrix unit's) with a conversion among them, beside 1,900 of
+// softmax, which the other's products slow by 1.4; without priority for the products it takes
+// 4,780 (the 1,640 rows 312 us for 305).  One wavefront a SIMD with 64 columns, softmax and products of two tiles in one
 // order, moved its sums between the two halves of the register file: 114 rows 200 us for 122.
 template <int HD>
 struct QsShape {

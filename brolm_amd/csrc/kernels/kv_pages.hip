@@ -800,6 +800,7 @@ int bx_qkv_append_q8_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k,
     if (rows <= 0 || n_q <= 0 || tab_rows <= 0 || k_stride < width || v_stride < width || q_stride < q_width ||
         q_out_stride < q_width)
         return fail(BX_EINVAL, "qkv_append_q8: bad shape");
+    if (q_out == q && q_out_stride != q_stride) return fail(BX_EINVAL, "qkv_append_q8: q_out over q at another stride");
     if (n_q > 1 << 24) return fail(BX_EUNSUPPORTED, "qkv_append_q8: too many rows and heads");
     if ((q_gain == nullptr) != (k_gain == nullptr)) return fail(BX_EINVAL, "qkv_append_q8: one of two gains");
     if (!(eps >= 0.f)) return fail(BX_EINVAL, "qkv_append_q8: bad eps");

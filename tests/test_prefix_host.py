@@ -45,7 +45,7 @@ QKV = [("q", P), ("q_stride", 2048), ("k", P), ("k_stride", 1024), ("v", P), ("v
     (dict(k_stride=1023), EINVAL, "shape"), (dict(v_stride=1), EINVAL, "shape"), (dict(q_out_stride=2047), EINVAL, "shape"),
     (dict(eps=-1.0), EINVAL, "eps"), (dict(eps=float("nan")), EINVAL, "eps"), (dict(n_kv=0), EINVAL, "cache shape"),
     (dict(n_pages=0), EINVAL, "cache shape"), (dict(page=48), EUNSUPPORTED, "pages hold"), (dict(hd=96), EUNSUPPORTED, "head_dim"),
-    (dict(vc=C.c_void_p(0x1008)), EINVAL, "aligned"),
+    (dict(vc=C.c_void_p(0x1008)), EINVAL, "aligned"), (dict(q_out_stride=2056), EINVAL, "another stride"),
     (dict(rows=2 ** 31 - 1, n_kv=64, k_stride=8192, v_stride=8192), EUNSUPPORTED, "too many"),
     (dict(n_q=(1 << 24) + 1, q_stride=1 << 32, q_out_stride=1 << 32), EUNSUPPORTED, "too many")])
 def test_qkv_append_refuses(native, kw, code, word):
